@@ -40,6 +40,8 @@ extern "C" {
 
 /* element type of weights / outputs / gradients / per-sample weights */
 enum { TBE_DTYPE_F32 = 0, TBE_DTYPE_F16 = 1, TBE_DTYPE_F64 = 2 };
+/* bfloat16: served by the expert-routing and gradient-clipping entry points; the others refuse it */
+enum { TBE_DTYPE_BF16 = 3 };
 
 /* optimizer selector of the entry points that serve several optimizers */
 enum {
@@ -624,6 +626,49 @@ TBE_API int tbe_backward_sgd_interleaved(const void *grad_output, void *weights,
                                          const int32_t *offsets, int32_t offsets_row_stride, int32_t B,
                                          float learning_rate, void *workspace, uint64_t workspace_bytes,
                                          void *stream);
+
+/* ------------------------------------------------------------ expert routing
+ * The rows of tokens in the order of the experts they chose, and back: the routed part of a mixture-of-experts
+ * layer.  No counterpart in the reference.  Token t of num_tokens chooses `choices` experts; pair
+ * a = t * choices + j names its j-th.  A pair whose expert lies outside [0, num_experts) is dropped: it takes
+ * part in nothing (its row, its weight and its gradient are not read), and its place is behind the last
+ * expert's rows.  num_experts <= 4095, num_tokens * choices < 2^31.
+ *
+ * tbe_expert_plan: a stable sort of the pairs by expert.
+ *   expert_ids      int32 or int64 (id_bytes = 4 or 8) [num_pairs]
+ *   expert_offsets  int32 [num_experts + 1]  first row of every expert, then the number of rows kept
+ *   order           int32 [num_pairs]  pair at every place: those of expert 0 first, then expert 1, ..., then the
+ *                                      dropped ones, ascending inside each
+ *   places          int32 [num_pairs]  the inverse: place of every pair
+ * The workspace (tbe_expert_plan_workspace_bytes; 0 for sizes that are refused) is free again after the call's
+ * launches.
+ *
+ * Rows have D elements of `dtype` (TBE_DTYPE_F32, F16, F64 or BF16); the *_stride arguments are the elements
+ * from one row of an input to the next (outputs are contiguous).  num_rows = num_tokens * choices.
+ *   dispatch          rows[places[a]] = tokens[a / choices], a row of zeros for a dropped pair
+ *   combine           output[t] = sum of weights[a] * rows[places[a]] over the kept pairs of t, added up in the
+ *                     order of j in 32 bits (64 for F64), rounded once; zeros for a token without kept pairs.
+ *                     weights: [num_rows], F32 or `dtype`; NULL = ones, which is dispatch's gradient
+ *   combine_backward  grad_rows[places[a]] = weights[a] * grad_output[t] (zeros for a dropped pair),
+ *                     grad_weights[a] = <rows[places[a]], grad_output[t]> (zero for a dropped pair)
+ * A place outside [0, num_rows) is treated as a dropped pair's and not written.  The calls only launch kernels
+ * on `stream`; they can be captured.
+ */
+TBE_API uint64_t tbe_expert_plan_workspace_bytes(int64_t num_pairs, int32_t num_experts);
+TBE_API int tbe_expert_plan(const void *expert_ids, int32_t id_bytes, int64_t num_pairs, int32_t num_experts,
+                    int32_t *expert_offsets, int32_t *order, int32_t *places, void *workspace,
+                    uint64_t workspace_bytes, void *stream);
+TBE_API int tbe_expert_dispatch(const void *tokens, int64_t token_stride, int32_t dtype, int64_t num_tokens,
+                    int32_t choices, int32_t num_experts, int64_t D, const int32_t *places,
+                    const int32_t *expert_offsets, void *rows, void *stream);
+TBE_API int tbe_expert_combine(const void *rows, int64_t row_stride, int32_t dtype, int64_t num_tokens,
+                    int32_t choices, int32_t num_experts, int64_t D, const int32_t *places,
+                    const int32_t *expert_offsets, const void *weights, int32_t weights_dtype, void *output,
+                    void *stream);
+TBE_API int tbe_expert_combine_backward(const void *grad_output, int64_t grad_stride, const void *rows,
+                    int64_t row_stride, int32_t dtype, int64_t num_tokens, int32_t choices, int32_t num_experts,
+                    int64_t D, const int32_t *places, const int32_t *expert_offsets, const void *weights,
+                    int32_t weights_dtype, void *grad_rows, void *grad_weights, void *stream);
 
 /* ------------------------------------------------------ host-resident tables
  * Pinned, device-mapped host memory (new_host_mapped_tensor,

@@ -20,7 +20,7 @@ BINDING_NAME = "table_batched_embeddings_cpp"
 BINDING_PATH = os.path.join(HERE, BINDING_NAME + ".so")
 BINDING_SOURCE = "table_batched_embeddings_binding.cpp"
 SOURCES = ["tbe_api.hip", "tbe_forward.hip", "tbe_sort.hip", "tbe_update.hip", "tbe_backward.hip",
-           "tbe_cache.hip", "tbe_mixed.hip", "tbe_approx.hip"]
+           "tbe_cache.hip", "tbe_mixed.hip", "tbe_approx.hip", "tbe_experts.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",

@@ -19,6 +19,8 @@ from torch import nn
 
 import table_batched_embeddings
 import table_batched_embeddings_cache
+from table_batched_embeddings_experts import (  # noqa: F401  (extensions, part of this module's surface)
+    ExpertRouting, expert_combine, expert_dispatch, expert_plan)
 
 # The module behind the ten functions that the reference imports as `table_batched_embeddings`
 # (table_batched_embeddings_ops.py:24, 53, 148): the Python binding of the C ABI by default, or the

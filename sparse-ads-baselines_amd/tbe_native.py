@@ -11,7 +11,9 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("TBE_HIP_LIBRARY") or os.path.join(_HERE, "libtbe_hip.so")
 
 DTYPE_F32, DTYPE_F16, DTYPE_F64 = 0, 1, 2
-ABI_VERSION = 22
+DTYPE_BF16 = 3  # expert routing and gradient clipping only
+ABI_VERSION = 23
+MAX_EXPERTS = 4095
 
 _c_i32p = ctypes.c_void_p
 _vp = ctypes.c_void_p
@@ -143,6 +145,13 @@ SIGNATURES = {
                                                 _c_i32p, _vp, _vp]),
     "tbe_backward_mixed_cached": (ctypes.c_int, [_i32, _vp, _cache_p, _i32, _i32, _i32, _i32, _i32, _i64, _c_i32p, _vp,
                                                  _vp, _f32, _f32, _vp, _i32, _u64, _u64, _vp, _u64, _c_i32p, _vp]),
+    "tbe_expert_plan_workspace_bytes": (_u64, [_i64, _i32]),
+    "tbe_expert_plan": (ctypes.c_int, [_vp, _i32, _i64, _i32, _c_i32p, _c_i32p, _c_i32p, _vp, _u64, _vp]),
+    "tbe_expert_dispatch": (ctypes.c_int, [_vp, _i64, _i32, _i64, _i32, _i32, _i64, _c_i32p, _c_i32p, _vp, _vp]),
+    "tbe_expert_combine": (ctypes.c_int, [_vp, _i64, _i32, _i64, _i32, _i32, _i64, _c_i32p, _c_i32p, _vp, _i32, _vp,
+                                          _vp]),
+    "tbe_expert_combine_backward": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i32, _i64, _i32, _i32, _i64, _c_i32p,
+                                                   _c_i32p, _vp, _i32, _vp, _vp, _vp]),
     "tbe_host_mapped_alloc": (ctypes.c_int, [_u64, ctypes.POINTER(_vp), ctypes.POINTER(_vp)]),
     "tbe_host_mapped_free": (ctypes.c_int, [_vp]),
     "tbe_managed_alloc": (ctypes.c_int, [_u64, _i32, ctypes.POINTER(_vp)]),
