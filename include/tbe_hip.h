@@ -632,7 +632,7 @@ TBE_API int tbe_backward_sgd_interleaved(const void *grad_output, void *weights,
  * layer.  No counterpart in the reference.  Token t of num_tokens chooses `choices` experts; pair
  * a = t * choices + j names its j-th.  A pair whose expert lies outside [0, num_experts) is dropped: it takes
  * part in nothing (its row, its weight and its gradient are not read), and its place is behind the last
- * expert's rows.  num_experts <= 4095, num_tokens * choices < 2^31.
+ * expert's rows.  num_experts <= TBE_MAX_EXPERTS, num_tokens * choices < 2^31.
  *
  * tbe_expert_plan: a stable sort of the pairs by expert.
  *   expert_ids      int32 or int64 (id_bytes = 4 or 8) [num_pairs]
@@ -650,10 +650,12 @@ TBE_API int tbe_backward_sgd_interleaved(const void *grad_output, void *weights,
  *                     order of j in 32 bits (64 for F64), rounded once; zeros for a token without kept pairs.
  *                     weights: [num_rows], F32 or `dtype`; NULL = ones, which is dispatch's gradient
  *   combine_backward  grad_rows[places[a]] = weights[a] * grad_output[t] (zeros for a dropped pair),
- *                     grad_weights[a] = <rows[places[a]], grad_output[t]> (zero for a dropped pair)
+ *                     grad_weights[a] = <rows[places[a]], grad_output[t]> (zero for a dropped pair);
+ *                     either may be NULL (without grad_weights, rows are not read and may be NULL too)
  * A place outside [0, num_rows) is treated as a dropped pair's and not written.  The calls only launch kernels
  * on `stream`; they can be captured.
  */
+#define TBE_MAX_EXPERTS 4095
 TBE_API uint64_t tbe_expert_plan_workspace_bytes(int64_t num_pairs, int32_t num_experts);
 TBE_API int tbe_expert_plan(const void *expert_ids, int32_t id_bytes, int64_t num_pairs, int32_t num_experts,
                     int32_t *expert_offsets, int32_t *order, int32_t *places, void *workspace,
@@ -669,6 +671,42 @@ TBE_API int tbe_expert_combine_backward(const void *grad_output, int64_t grad_st
                     int64_t row_stride, int32_t dtype, int64_t num_tokens, int32_t choices, int32_t num_experts,
                     int64_t D, const int32_t *places, const int32_t *expert_offsets, const void *weights,
                     int32_t weights_dtype, void *grad_rows, void *grad_weights, void *stream);
+
+/* ------------------------------------------------- gradient norm and clipping
+ * The global norm of a list of gradients, N = sqrt(sum of g^2 over all of them), and the gradients scaled by
+ * min(1, max_norm / (N + 1e-6)).  No counterpart in the reference, which leaves clipping to PyTorch.
+ *
+ * gradients, outputs, numels and dtypes are HOST arrays of num_tensors entries (device addresses, element counts,
+ * F32 / F16 / F64 / BF16); the tensors are dense and need no more alignment than their elements'.  An empty
+ * tensor's pointers may be null.  `norm` is one F32 or F64 value in device memory.
+ *   tbe_gradient_norm    writes the norm: squares added up in 64 bits, rounded once
+ *   tbe_scale_gradients  reads it: outputs[i] = gradients[i] * min(1, max_norm / (*norm + 1e-6)), with a
+ *                        product in 32 bits (64 for F64).  A norm that is not a number makes every output one;
+ *                        an infinite norm makes finite gradients zero.
+ *   tbe_clip_gradients   the two in a row
+ * outputs[i] may be gradients[i] (in place: nothing is written while the norm is within max_norm); any other
+ * overlap of an output with a tensor of the list is refused.  max_norm >= 0 (infinity: nothing is scaled).
+ * The workspace serves one call at a time.  The calls only launch kernels on `stream`; they can be captured
+ * (the addresses and counts are part of the captured launches).
+ *
+ * tbe_table_gradient_norm writes the norm of the exact gradient of a batch's tables -- one row per distinct
+ * (table, index), the sum over its lookups of (per_sample_weights[p] *) grad_output[bag(p)] -- from the workspace
+ * that tbe_plan_batch (same D, dtype, T, B and num_indices) has filled.  It leaves the plan as it is: a
+ * tbe_backward_planned may follow, with the same or a scaled grad_output.
+ */
+TBE_API uint64_t tbe_gradient_norm_workspace_bytes(int32_t num_tensors);
+TBE_API int tbe_gradient_norm(const void *const *gradients, const int64_t *numels, const int32_t *dtypes,
+                      int32_t num_tensors, void *norm, int32_t norm_dtype, void *workspace,
+                      uint64_t workspace_bytes, void *stream);
+TBE_API int tbe_scale_gradients(const void *const *gradients, void *const *outputs, const int64_t *numels,
+                      const int32_t *dtypes, int32_t num_tensors, double max_norm, const void *norm,
+                      int32_t norm_dtype, void *stream);
+TBE_API int tbe_clip_gradients(const void *const *gradients, void *const *outputs, const int64_t *numels,
+                      const int32_t *dtypes, int32_t num_tensors, double max_norm, void *norm, int32_t norm_dtype,
+                      void *workspace, uint64_t workspace_bytes, void *stream);
+TBE_API int tbe_table_gradient_norm(const void *grad_output, int32_t dtype, int32_t D, int32_t T, int32_t B,
+                      int64_t num_indices, const void *per_sample_weights, void *workspace,
+                      uint64_t workspace_bytes, void *norm, int32_t norm_dtype, void *stream);
 
 /* ------------------------------------------------------ host-resident tables
  * Pinned, device-mapped host memory (new_host_mapped_tensor,

@@ -18,9 +18,10 @@ LIB_NAME = "libtbe_hip.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 BINDING_NAME = "table_batched_embeddings_cpp"
 BINDING_PATH = os.path.join(HERE, BINDING_NAME + ".so")
-BINDING_SOURCE = "table_batched_embeddings_binding.cpp"
+BINDING_SOURCES = ["table_batched_embeddings_binding.cpp", "table_batched_embeddings_training.cpp"]
 SOURCES = ["tbe_api.hip", "tbe_forward.hip", "tbe_sort.hip", "tbe_update.hip", "tbe_backward.hip",
-           "tbe_cache.hip", "tbe_mixed.hip", "tbe_approx.hip", "tbe_experts.hip"]
+           "tbe_cache.hip", "tbe_mixed.hip", "tbe_approx.hip", "tbe_experts.hip",
+           "tbe_clip.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",
@@ -79,16 +80,17 @@ def build(verbose=False):
 
 
 def build_binding(verbose=False):
-    """Compiles the pybind11 module (BINDING_SOURCE) and links it against LIB_PATH and PyTorch.
+    """Compiles the pybind11 module (BINDING_SOURCES, in parallel) and links it against LIB_PATH and PyTorch.
     It finds the library next to itself (rpath $ORIGIN)."""
     import sysconfig
 
     import torch
     from torch.utils import cpp_extension
 
-    source = os.path.join(CSRC, BINDING_SOURCE)
-    if not os.path.exists(source):
-        raise RuntimeError("missing source %s" % source)
+    sources = [os.path.join(CSRC, s) for s in BINDING_SOURCES]
+    for source in sources:
+        if not os.path.exists(source):
+            raise RuntimeError("missing source %s" % source)
     gxx = shutil.which("g++")
     if gxx is None:
         raise RuntimeError("g++ not found; the pybind11 module needs a host C++ compiler")
@@ -96,13 +98,20 @@ def build_binding(verbose=False):
     includes = [os.path.join(os.path.dirname(HERE), "include")] + cpp_extension.include_paths() + \
         ["/opt/rocm/include", sysconfig.get_paths()["include"]]
     tmp = BINDING_PATH + ".tmp"
-    cmd = [gxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-           "-DTORCH_EXTENSION_NAME=" + BINDING_NAME, "-DTORCH_API_INCLUDE_EXTENSION_H",
-           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-w"]
-    cmd += ["-I" + d for d in includes]
-    cmd += [source, "-o", tmp, "-L" + torch_lib, "-L" + HERE, "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10",
-            "-lc10_hip", "-ltorch_hip", "-ltbe_hip", "-Wl,-rpath,$ORIGIN"]
-    out = _run(cmd)
+    flags = ["-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+             "-DTORCH_EXTENSION_NAME=" + BINDING_NAME, "-DTORCH_API_INCLUDE_EXTENSION_H",
+             "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-w"]
+    flags += ["-I" + d for d in includes]
+    obj_dir = os.path.join(HERE, "build")
+    os.makedirs(obj_dir, exist_ok=True)
+    objects = [os.path.join(obj_dir, os.path.basename(s).replace(".cpp", ".o")) for s in sources]
+    with concurrent.futures.ThreadPoolExecutor(len(sources)) as pool:
+        outputs = list(pool.map(lambda pair: _run([gxx] + flags + ["-c", pair[0], "-o", pair[1]]),
+                                zip(sources, objects)))
+    outputs.append(_run([gxx, "-shared", "-o", tmp] + objects + [
+        "-L" + torch_lib, "-L" + HERE, "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip", "-ltorch_hip",
+        "-ltbe_hip", "-Wl,-rpath,$ORIGIN"]))
+    out = "\n".join(outputs)
     os.replace(tmp, BINDING_PATH)
     if verbose and out.strip():
         print(out)

@@ -24,9 +24,9 @@
 #include <utility>
 #include <vector>
 
-#include "tbe_hip.h"
+#include "table_batched_embeddings_binding.h"
 
-namespace {
+namespace tbe_binding {
 
 void check(int rc) {
   TORCH_CHECK(rc == TBE_OK, tbe_last_error());
@@ -47,11 +47,6 @@ void *stream_of(const at::Tensor &t) {
 }
 
 const void *ptr(const c10::optional<at::Tensor> &t) { return t.has_value() ? t->data_ptr() : nullptr; }
-
-struct Shape {
-  int32_t T, B, D;
-  int64_t n, rows;
-};
 
 // table_batched_embeddings_cuda.cu:262-273 (AT_ASSERT on T, B, D) plus the dtype / device /
 // contiguity checks that at::Tensor accessors make there.
@@ -114,16 +109,9 @@ struct HeldWorkspace {
   std::shared_ptr<std::mutex> busy = std::make_shared<std::mutex>();
   uint64_t last_use = 0;
 };
-struct Scratch {
-  at::Tensor tensor;
-  std::shared_ptr<std::mutex> busy;
-  std::unique_lock<std::mutex> lock;
-  void *data() const { return tensor.data_ptr(); }
-  uint64_t bytes() const { return static_cast<uint64_t>(tensor.numel()); }
-};
-std::mutex g_workspaces_mutex;
-std::map<std::pair<int, void *>, HeldWorkspace> g_workspaces;
-uint64_t g_workspace_clock = 0;
+static std::mutex g_workspaces_mutex;
+static std::map<std::pair<int, void *>, HeldWorkspace> g_workspaces;
+static uint64_t g_workspace_clock = 0;
 
 Scratch workspace(const at::Tensor &like, uint64_t bytes) {
   const std::pair<int, void *> key{static_cast<int>(like.get_device()), stream_of(like)};
@@ -499,9 +487,10 @@ at::Tensor new_host_mapped_tensor(at::Tensor self, std::vector<int64_t> sizes) {
   return at::from_blob(device, sizes, [host](void *) { tbe_host_mapped_free(host); }, self.options(), self.device());
 }
 
-}  // namespace
+}  // namespace tbe_binding
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  using namespace tbe_binding;
   m.def("forward", &forward, "forward");
   m.def("backward_sgd", &backward_sgd, "backward_sgd");
   m.def("backward_exact_adagrad", &backward_exact_adagrad, "backward_exact_adagrad");
@@ -515,4 +504,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("abi_version", []() { return tbe_abi_version(); }, "version of the C ABI the library exports");
   m.def("reserve_workspace", &reserve_workspace, "sizes the current stream's scratch tensor ahead of time");
   m.def("release_workspaces", &release_workspaces, "drops the scratch tensors the module holds");
+  bind_training(m);
 }

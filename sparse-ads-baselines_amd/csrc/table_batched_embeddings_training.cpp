@@ -1,0 +1,382 @@
+// Expert routing, gradient clipping and the clipped table updates of the pybind11 module
+// table_batched_embeddings_cpp (no counterpart in the reference).  Host code over the C ABI: checks, outputs,
+// autograd; the kernels are in the library.  The smallest calls are bound by what the host does for them,
+// which is why these operators live here and not in the ctypes module.
+//
+// Scratch memory that a call needs comes from PyTorch's allocator for that call alone, except for the sort
+// workspace of a clipped table update, which is the stream's like that of every other update.
+#include "table_batched_embeddings_binding.h"
+
+#include <torch/csrc/autograd/custom_function.h>
+
+#include <c10/core/DeviceGuard.h>
+
+#include <limits>
+#include <tuple>
+#include <vector>
+
+namespace tbe_binding {
+namespace {
+
+// element types of expert routing and clipping: those of the tables and bfloat16
+int32_t float_code(const at::Tensor &t, const char *name) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return TBE_DTYPE_F32;
+    case at::kHalf: return TBE_DTYPE_F16;
+    case at::kDouble: return TBE_DTYPE_F64;
+    case at::kBFloat16: return TBE_DTYPE_BF16;
+    default: TORCH_CHECK(false, name, " must be float16, bfloat16, float32 or float64");
+  }
+  return -1;
+}
+
+// ------------------------------------------------------------------------------ expert routing
+struct Plan {
+  int64_t tokens;
+  int32_t choices, experts;
+};
+
+Plan check_plan(const at::Tensor &places, const at::Tensor &expert_offsets, const at::Device &device) {
+  TORCH_CHECK(places.scalar_type() == at::kInt && expert_offsets.scalar_type() == at::kInt,
+              "places and expert_offsets must be int32");
+  TORCH_CHECK(places.device() == device && expert_offsets.device() == device,
+              "places and expert_offsets must live on the rows' device");
+  TORCH_CHECK(places.dim() == 2 && places.is_contiguous() && places.size(1) > 0,
+              "places must be a contiguous [tokens, choices] tensor with choices > 0");
+  TORCH_CHECK(expert_offsets.dim() == 1 && expert_offsets.is_contiguous() && expert_offsets.numel() > 1,
+              "expert_offsets must be a contiguous 1-D tensor of num_experts + 1 entries");
+  TORCH_CHECK(places.numel() < std::numeric_limits<int32_t>::max() &&
+                  expert_offsets.numel() < std::numeric_limits<int32_t>::max(),
+              "tokens * choices must stay below 2^31 - 1");
+  return Plan{places.size(0), static_cast<int32_t>(places.size(1)), static_cast<int32_t>(expert_offsets.numel() - 1)};
+}
+
+// Rows at any distance from each other are read in place; anything else is laid out first.
+at::Tensor check_rows(const at::Tensor &rows, const char *name, int64_t count) {
+  TORCH_CHECK(rows.is_cuda(), name, " must be a GPU tensor");
+  TORCH_CHECK(rows.dim() == 2 && rows.size(1) > 0, name, " must be a [rows, D] tensor with D > 0");
+  TORCH_CHECK(rows.size(0) == count, name, " must have ", count, " rows (one row per row of places, or per pair), got ",
+              rows.size(0));
+  return rows.stride(1) == 1 && rows.stride(0) >= 0 ? rows : rows.contiguous();
+}
+int64_t row_stride(const at::Tensor &rows) { return rows.size(0) > 1 ? rows.stride(0) : rows.size(1); }
+
+at::Tensor check_gates(const at::Tensor &weights, const at::Tensor &rows, const at::Tensor &places) {
+  TORCH_CHECK(weights.scalar_type() == rows.scalar_type() || weights.scalar_type() == at::kFloat,
+              "weights must be float32 or have the rows' dtype");
+  TORCH_CHECK(weights.device() == rows.device(), "weights must live on the rows' device");
+  TORCH_CHECK(weights.sizes() == places.sizes(), "weights must be [tokens, choices]");
+  return weights.contiguous();
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> expert_plan(at::Tensor expert_ids, int64_t num_experts) {
+  TORCH_CHECK(expert_ids.is_cuda(), "expert_ids must be a GPU tensor");
+  TORCH_CHECK(expert_ids.scalar_type() == at::kInt || expert_ids.scalar_type() == at::kLong,
+              "expert_ids must be int32 or int64");
+  TORCH_CHECK(expert_ids.dim() == 2 && expert_ids.size(1) > 0, "expert_ids must be [tokens, choices] with choices > 0");
+  const int64_t pairs = expert_ids.numel();
+  TORCH_CHECK(pairs < std::numeric_limits<int32_t>::max(), "tokens * choices must stay below 2^31 - 1");
+  TORCH_CHECK(num_experts > 0 && num_experts <= TBE_MAX_EXPERTS, "num_experts must be 1 to ", TBE_MAX_EXPERTS, " (got ",
+              num_experts, ")");
+  c10::DeviceGuard guard(expert_ids.device());
+  expert_ids = expert_ids.contiguous();
+  const auto ints = expert_ids.options().dtype(at::kInt);
+  at::Tensor expert_offsets = at::empty({num_experts + 1}, ints);
+  at::Tensor order = at::empty({pairs}, ints);
+  at::Tensor places = at::empty(expert_ids.sizes(), ints);
+  const uint64_t bytes = tbe_expert_plan_workspace_bytes(pairs, static_cast<int32_t>(num_experts));
+  // (a call of its own scratch: two graphs captured on one stream do not share it)
+  at::Tensor scratch = at::empty({static_cast<int64_t>(bytes)}, expert_ids.options().dtype(at::kByte));
+  check(tbe_expert_plan(expert_ids.data_ptr(), static_cast<int32_t>(expert_ids.element_size()), pairs,
+                        static_cast<int32_t>(num_experts), expert_offsets.data_ptr<int32_t>(),
+                        order.data_ptr<int32_t>(), places.data_ptr<int32_t>(), scratch.data_ptr(), bytes,
+                        stream_of(expert_ids)));
+  return {expert_offsets, order, places};
+}
+
+at::Tensor dispatch(const at::Tensor &tokens_in, const at::Tensor &places, const at::Tensor &expert_offsets) {
+  const at::Tensor tokens = check_rows(tokens_in, "tokens", places.dim() > 0 ? places.size(0) : 0);
+  const Plan p = check_plan(places, expert_offsets, tokens.device());
+  const int32_t dtype = float_code(tokens, "tokens");
+  c10::DeviceGuard guard(tokens.device());
+  at::Tensor rows = at::empty({p.tokens * p.choices, tokens.size(1)}, tokens.options());
+  check(tbe_expert_dispatch(tokens.data_ptr(), row_stride(tokens), dtype, p.tokens, p.choices, p.experts, tokens.size(1),
+                            places.data_ptr<int32_t>(), expert_offsets.data_ptr<int32_t>(), rows.data_ptr(),
+                            stream_of(tokens)));
+  return rows;
+}
+
+at::Tensor combine(const at::Tensor &rows_in, const at::Tensor &places, const at::Tensor &expert_offsets,
+                   const c10::optional<at::Tensor> &weights_in) {
+  const at::Tensor rows = check_rows(rows_in, "rows", places.numel());
+  const Plan p = check_plan(places, expert_offsets, rows.device());
+  const int32_t dtype = float_code(rows, "rows");
+  c10::optional<at::Tensor> weights;
+  if (weights_in.has_value()) weights = check_gates(*weights_in, rows, places);
+  c10::DeviceGuard guard(rows.device());
+  at::Tensor output = at::empty({p.tokens, rows.size(1)}, rows.options());
+  check(tbe_expert_combine(rows.data_ptr(), row_stride(rows), dtype, p.tokens, p.choices, p.experts, rows.size(1),
+                           places.data_ptr<int32_t>(), expert_offsets.data_ptr<int32_t>(), ptr(weights),
+                           weights.has_value() ? float_code(*weights, "weights") : dtype, output.data_ptr(),
+                           stream_of(rows)));
+  return output;
+}
+
+// (gradient of the rows, gradient of the weights), either of them only where it is wanted
+std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>> combine_backward(
+    const at::Tensor &grad_in, const at::Tensor &rows_in, const at::Tensor &places, const at::Tensor &expert_offsets,
+    const at::Tensor &weights_in, bool want_rows, bool want_weights) {
+  const at::Tensor rows = check_rows(rows_in, "rows", places.numel());
+  const Plan p = check_plan(places, expert_offsets, rows.device());
+  const int32_t dtype = float_code(rows, "rows");
+  const at::Tensor weights = check_gates(weights_in, rows, places);
+  TORCH_CHECK(grad_in.scalar_type() == rows.scalar_type(), "grad_output must have the rows' dtype");
+  TORCH_CHECK(grad_in.device() == rows.device(), "grad_output must live on the rows' device");
+  TORCH_CHECK(grad_in.dim() == 2 && grad_in.size(0) == p.tokens && grad_in.size(1) == rows.size(1),
+              "grad_output must be [tokens, D]");
+  const at::Tensor grad = check_rows(grad_in, "grad_output", p.tokens);
+  c10::DeviceGuard guard(rows.device());
+  c10::optional<at::Tensor> grad_rows, grad_weights;
+  if (want_rows) grad_rows = at::empty({rows.size(0), rows.size(1)}, rows.options());
+  if (want_weights) grad_weights = at::empty(places.sizes(), weights.options());
+  if (!want_rows && !want_weights) return {grad_rows, grad_weights};
+  check(tbe_expert_combine_backward(
+      grad.data_ptr(), row_stride(grad), rows.data_ptr(), row_stride(rows), dtype, p.tokens, p.choices, p.experts,
+      rows.size(1), places.data_ptr<int32_t>(), expert_offsets.data_ptr<int32_t>(), weights.data_ptr(),
+      float_code(weights, "weights"), const_cast<void *>(ptr(grad_rows)), const_cast<void *>(ptr(grad_weights)),
+      stream_of(rows)));
+  return {grad_rows, grad_weights};
+}
+
+// The kernels' results carry no graph of their own, so that a second derivative would silently be a wrong one.
+void refuse_second_derivative() {
+  TORCH_CHECK(!at::GradMode::is_enabled(), "expert routing is differentiable once (create_graph=True is not served)");
+}
+
+struct Dispatch : torch::autograd::Function<Dispatch> {
+  static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &tokens, const at::Tensor &places,
+                            const at::Tensor &expert_offsets) {
+    ctx->save_for_backward({places, expert_offsets});
+    return dispatch(tokens, places, expert_offsets);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
+                                                 torch::autograd::variable_list grads) {
+    refuse_second_derivative();
+    const auto saved = ctx->get_saved_variables();
+    return {combine(grads[0], saved[0], saved[1], c10::nullopt), at::Tensor(), at::Tensor()};
+  }
+};
+
+struct Combine : torch::autograd::Function<Combine> {
+  static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &rows, const at::Tensor &places,
+                            const at::Tensor &expert_offsets, const c10::optional<at::Tensor> &weights) {
+    ctx->saved_data["weighted"] = weights.has_value();
+    if (weights.has_value()) ctx->save_for_backward({rows, places, expert_offsets, *weights});
+    else ctx->save_for_backward({places, expert_offsets});
+    return combine(rows, places, expert_offsets, weights);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
+                                                 torch::autograd::variable_list grads) {
+    refuse_second_derivative();
+    const auto saved = ctx->get_saved_variables();
+    if (!ctx->saved_data["weighted"].toBool())
+      return {dispatch(grads[0], saved[0], saved[1]), at::Tensor(), at::Tensor(), at::Tensor()};
+    const auto wanted = combine_backward(grads[0], saved[0], saved[1], saved[2], saved[3], ctx->needs_input_grad(0),
+                                         ctx->needs_input_grad(3));
+    return {std::get<0>(wanted).value_or(at::Tensor()), at::Tensor(), at::Tensor(),
+            std::get<1>(wanted).value_or(at::Tensor())};
+  }
+};
+
+at::Tensor expert_dispatch(const at::Tensor &tokens, const at::Tensor &places, const at::Tensor &expert_offsets) {
+  if (at::GradMode::is_enabled() && tokens.requires_grad()) return Dispatch::apply(tokens, places, expert_offsets);
+  return dispatch(tokens, places, expert_offsets);
+}
+
+at::Tensor expert_combine(const at::Tensor &rows, const at::Tensor &places, const at::Tensor &expert_offsets,
+                          const c10::optional<at::Tensor> &weights) {
+  if (at::GradMode::is_enabled() && (rows.requires_grad() || (weights.has_value() && weights->requires_grad())))
+    return Combine::apply(rows, places, expert_offsets, weights);
+  return combine(rows, places, expert_offsets, weights);
+}
+
+// -------------------------------------------------------------------- gradient norm and clipping
+struct GradientList {
+  std::vector<const void *> gradients;
+  std::vector<void *> outputs;
+  std::vector<int64_t> numels;
+  std::vector<int32_t> dtypes;
+  bool f64 = false;
+  int32_t count() const { return static_cast<int32_t>(gradients.size()); }
+};
+
+GradientList check_gradients(const std::vector<at::Tensor> &gradients, const std::vector<at::Tensor> *outputs) {
+  TORCH_CHECK(!gradients.empty(), "there must be at least one gradient");
+  TORCH_CHECK(gradients.size() < (1u << 24), "too many gradients");
+  TORCH_CHECK(!outputs || outputs->size() == gradients.size(), "out must hold one tensor per gradient");
+  GradientList list;
+  list.gradients.reserve(gradients.size());
+  list.numels.reserve(gradients.size());
+  list.dtypes.reserve(gradients.size());
+  list.outputs.reserve(gradients.size());
+  const at::Device device = gradients[0].device();
+  for (size_t i = 0; i < gradients.size(); ++i) {
+    const at::Tensor &g = gradients[i];
+    TORCH_CHECK(g.is_cuda(), "gradients must be GPU tensors");
+    TORCH_CHECK(g.layout() == at::kStrided, "gradients must be strided (dense) tensors");
+    TORCH_CHECK(g.device() == device, "gradients must live on one device");
+    // (any order of the dimensions, transposed ones among them: the elements are one block of memory)
+    TORCH_CHECK(g.is_non_overlapping_and_dense(), "gradients must be dense: gradient ", i, " has gaps or repeats elements");
+    list.dtypes.push_back(float_code(g, "gradients"));
+    list.f64 = list.f64 || g.scalar_type() == at::kDouble;
+    list.gradients.push_back(g.data_ptr());
+    list.numels.push_back(g.numel());
+    const at::Tensor &o = outputs ? (*outputs)[i] : g;
+    if (outputs)
+      TORCH_CHECK(o.device() == device && o.scalar_type() == g.scalar_type() && o.sizes() == g.sizes() &&
+                      o.strides() == g.strides(),
+                  "out must have the gradients' shapes, strides, types and device (tensor ", i, ")");
+    list.outputs.push_back(o.data_ptr());
+  }
+  return list;
+}
+
+at::Tensor empty_norm(const at::Tensor &like, bool f64) {
+  return at::empty({}, like.options().dtype(f64 ? at::kDouble : at::kFloat));
+}
+int32_t norm_code(bool f64) { return f64 ? TBE_DTYPE_F64 : TBE_DTYPE_F32; }
+
+at::Tensor gradient_norm(const std::vector<at::Tensor> &gradients) {
+  const GradientList list = check_gradients(gradients, nullptr);
+  c10::DeviceGuard guard(gradients[0].device());
+  at::Tensor norm = empty_norm(gradients[0], list.f64);
+  const uint64_t bytes = tbe_gradient_norm_workspace_bytes(list.count());
+  at::Tensor scratch = at::empty({static_cast<int64_t>(bytes)}, gradients[0].options().dtype(at::kByte));
+  check(tbe_gradient_norm(list.gradients.data(), list.numels.data(), list.dtypes.data(), list.count(), norm.data_ptr(),
+                          norm_code(list.f64), scratch.data_ptr(), bytes, stream_of(gradients[0])));
+  return norm;
+}
+
+at::Tensor clip_gradients(const std::vector<at::Tensor> &gradients, double max_norm,
+                          const c10::optional<std::vector<at::Tensor>> &out) {
+  const GradientList list = check_gradients(gradients, out.has_value() ? &*out : nullptr);
+  TORCH_CHECK(max_norm >= 0.0, "max_norm must not be negative");
+  c10::DeviceGuard guard(gradients[0].device());
+  at::Tensor norm = empty_norm(gradients[0], list.f64);
+  const uint64_t bytes = tbe_gradient_norm_workspace_bytes(list.count());
+  at::Tensor scratch = at::empty({static_cast<int64_t>(bytes)}, gradients[0].options().dtype(at::kByte));
+  check(tbe_clip_gradients(list.gradients.data(), list.outputs.data(), list.numels.data(), list.dtypes.data(),
+                           list.count(), max_norm, norm.data_ptr(), norm_code(list.f64), scratch.data_ptr(), bytes,
+                           stream_of(gradients[0])));
+  // autograd learns that the tensors were written
+  for (const at::Tensor &t : out.has_value() ? *out : gradients)
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  return norm;
+}
+
+// ------------------------------------------------------------------------ clipped table updates
+struct TableClip {
+  at::Tensor clipped, norm;
+};
+
+// The batch's plan into `ws`, the norm of the tables' exact gradient, and grad_output scaled by it.
+TableClip plan_and_clip(const at::Tensor &grad_output, const at::Tensor &weights, const at::Tensor &table_offsets,
+                        const at::Tensor &indices, const at::Tensor &offsets,
+                        const c10::optional<at::Tensor> &indice_weights, const Shape &s, int32_t dtype, double max_norm,
+                        const Scratch &ws) {
+  const bool f64 = weights.scalar_type() == at::kDouble;
+  TableClip clip{at::empty_like(grad_output), empty_norm(weights, f64)};
+  void *stream = stream_of(weights);
+  check(tbe_plan_batch(table_offsets.data_ptr<int32_t>(), s.T, indices.data_ptr<int32_t>(), s.n,
+                       offsets.data_ptr<int32_t>(), s.B, s.rows, max_table_rows(table_offsets, s.rows), s.D, dtype,
+                       ws.data(), ws.bytes(), stream));
+  check(tbe_table_gradient_norm(grad_output.data_ptr(), dtype, s.D, s.T, s.B, s.n, ptr(indice_weights), ws.data(),
+                                ws.bytes(), clip.norm.data_ptr(), norm_code(f64), stream));
+  const void *gradient = grad_output.data_ptr();
+  void *output = clip.clipped.data_ptr();
+  const int64_t numel = grad_output.numel();
+  check(tbe_scale_gradients(&gradient, &output, &numel, &dtype, 1, max_norm, clip.norm.data_ptr(), norm_code(f64), stream));
+  return clip;
+}
+
+uint64_t plan_bytes(const Shape &s, int32_t dtype) {
+  tbe_workspace_layout_t layout;
+  check(tbe_backward_workspace_layout(s.n, s.D, dtype, s.T, &layout));
+  return layout.total_bytes;
+}
+
+std::tuple<at::Tensor, at::Tensor> clip_table_gradient(at::Tensor grad_output, at::Tensor weights,
+                                                       at::Tensor table_offsets, at::Tensor indices, at::Tensor offsets,
+                                                       double max_norm, c10::optional<at::Tensor> indice_weights) {
+  const Shape s = check_common(weights, table_offsets, indices, offsets);
+  grad_output = check_grad(grad_output, weights, s);
+  check_weights_of_lookups(indice_weights, weights, indices);
+  TORCH_CHECK(max_norm >= 0.0, "max_norm must not be negative");
+  const int32_t dtype = dtype_code(weights);
+  c10::DeviceGuard guard(weights.device());
+  const Scratch ws = workspace(weights, plan_bytes(s, dtype));
+  const TableClip clip = plan_and_clip(grad_output, weights, table_offsets, indices, offsets, indice_weights, s, dtype,
+                                       max_norm, ws);
+  return {clip.clipped, clip.norm};
+}
+
+// backward_sgd / backward_exact_adagrad on the clipped gradient, one plan for the norm and the update.
+at::Tensor backward_clipped(int64_t optimizer, at::Tensor grad_output, at::Tensor weights, at::Tensor table_offsets,
+                            at::Tensor indices, at::Tensor offsets, c10::optional<at::Tensor> indice_weights,
+                            c10::optional<at::Tensor> optimizer_state, double learning_rate, double eps,
+                            bool stochastic_rounding, double max_norm) {
+  const Shape s = check_common(weights, table_offsets, indices, offsets);
+  grad_output = check_grad(grad_output, weights, s);
+  check_weights_of_lookups(indice_weights, weights, indices);
+  TORCH_CHECK(max_norm >= 0.0, "max_norm must not be negative");
+  TORCH_CHECK(optimizer == TBE_OPT_SGD || optimizer == TBE_OPT_ROWWISE_ADAGRAD, "optimizer must be SGD or row-wise Adagrad");
+  const bool adagrad = optimizer == TBE_OPT_ROWWISE_ADAGRAD;
+  TORCH_CHECK(adagrad || !indice_weights.has_value(), "SGD takes no per-sample weights");
+  TORCH_CHECK(!adagrad || optimizer_state.has_value(), "row-wise Adagrad needs its state");
+  if (adagrad) check_state(*optimizer_state, weights);
+  const int32_t dtype = dtype_code(weights);
+  c10::DeviceGuard guard(weights.device());
+  const bool rounds = adagrad && stochastic_rounding && weights.scalar_type() == at::kHalf;
+  std::pair<uint64_t, uint64_t> stream_of_bits{0, 0};
+  if (rounds) stream_of_bits = rounding_stream(weights);  // (takes the interpreter's lock: before the workspace's)
+  const Scratch ws = workspace(weights, plan_bytes(s, dtype));
+  const TableClip clip = plan_and_clip(grad_output, weights, table_offsets, indices, offsets, indice_weights, s, dtype,
+                                       max_norm, ws);
+  // (the clipped gradient's dot products with the rows, which nobody asks for: the update writes them)
+  c10::optional<at::Tensor> unused;
+  if (indice_weights.has_value()) unused = at::empty_like(*indice_weights);
+  check(tbe_backward_planned(static_cast<int32_t>(optimizer), clip.clipped.data_ptr(), weights.data_ptr(), dtype, s.rows,
+                             s.D, s.T, s.B, s.n, ptr(indice_weights), adagrad ? optimizer_state->data_ptr() : nullptr,
+                             static_cast<float>(learning_rate), static_cast<float>(eps),
+                             const_cast<void *>(ptr(unused)), rounds ? 1 : 0, stream_of_bits.first,
+                             stream_of_bits.second, ws.data(), ws.bytes(), stream_of(weights)));
+  return clip.norm;
+}
+
+}  // namespace
+
+void bind_training(pybind11::module &m) {
+  namespace py = pybind11;
+  using release = py::call_guard<py::gil_scoped_release>;
+  m.def("expert_plan", &expert_plan, "stable order of the (token, choice) pairs by expert", py::arg("expert_ids"),
+        py::arg("num_experts"), release());
+  m.def("expert_dispatch", &expert_dispatch, "rows of the tokens in expert order", py::arg("tokens"), py::arg("places"),
+        py::arg("expert_offsets"), release());
+  m.def("expert_combine", &expert_combine, "weighted sums of the experts' rows in token order", py::arg("rows"),
+        py::arg("places"), py::arg("expert_offsets"), py::arg("weights") = py::none(), release());
+  m.def("expert_combine_backward", &combine_backward, "gradients of expert_combine", py::arg("grad_output"),
+        py::arg("rows"), py::arg("places"), py::arg("expert_offsets"), py::arg("weights"), py::arg("want_rows") = true,
+        py::arg("want_weights") = true, release());
+  m.def("gradient_norm", &gradient_norm, "global norm of a list of gradients", py::arg("gradients"), release());
+  m.def("clip_gradients", &clip_gradients, "scales a list of gradients down to a global norm", py::arg("gradients"),
+        py::arg("max_norm"), py::arg("out") = py::none(), release());
+  m.def("clip_table_gradient", &clip_table_gradient, "grad_output scaled by the norm of the tables' exact gradient",
+        py::arg("grad_output"), py::arg("weights"), py::arg("table_offsets"), py::arg("indices"), py::arg("offsets"),
+        py::arg("max_norm"), py::arg("indice_weights") = py::none(), release());
+  m.def("backward_clipped", &backward_clipped, "table update with the clipped gradient", py::arg("optimizer"),
+        py::arg("grad_output"), py::arg("weights"), py::arg("table_offsets"), py::arg("indices"), py::arg("offsets"),
+        py::arg("indice_weights"), py::arg("optimizer_state"), py::arg("learning_rate"), py::arg("eps"),
+        py::arg("stochastic_rounding"), py::arg("max_norm"), release());
+}
+
+}  // namespace tbe_binding

@@ -1,0 +1,653 @@
+// The global norm of gradients and clipping to it, for gfx950:
+//   norm    N = sqrt(sum over all tensors and elements of g^2)
+//   scaled  g * min(1, max_norm / (N + 1e-6)), a NaN of the quotient kept
+// and, for a sorted batch of embedding lookups, the norm of the tables' exact gradient, which has one row
+// per distinct index and is never stored:
+//   N = sqrt(sum over rows r of || sum over lookups p of row r of (w_p *) g[bag(p)] ||^2)
+// Squares are added up in 64 bits: no value that a 32-bit float holds overflows there, and the memory system,
+// not the vector ALU, stays what these passes wait for.  Every sum has one fixed order (no atomics), so two runs
+// of the same lists are bit-identical.
+
+#include <algorithm>
+#include <new>
+#include <utility>
+#include <vector>
+
+#include "tbe_stages.h"
+
+namespace tbe {
+namespace {
+
+// ------------------------------------------------------------------------------ lists of tensors
+// A launch takes up to kListTensors tensors of one type by kernel argument (under 4 KB).  A tensor is cut into
+// chunks of whole 16-byte vectors, counted from the 16-byte boundary at or before its first element: the
+// first and the last vector of a tensor may be partly outside it and are then taken element by element.
+constexpr int kListTensors = 128;
+struct TensorList {
+  const void *src[kListTensors];
+  void *dst[kListTensors];
+  int64_t numel[kListTensors];
+  int32_t chunk_end[kListTensors];  // running number of chunks
+  int32_t count;
+  int32_t chunks;
+  int32_t chunk_vectors;
+};
+
+__device__ __forceinline__ int tensor_of_chunk(const TensorList &list, int chunk) {
+  int lo = 0, hi = list.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (chunk < list.chunk_end[mid]) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
+}
+
+template <typename T> struct alignas(16) Vec16 {
+  static constexpr int kCount = 16 / sizeof(T);
+  T v[kCount];
+};
+
+// What the lanes of this wavefront have written to LDS is there for its other lanes.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+  for (int m = 1; m < kWave; m <<= 1) v += shfl_x(v, m);
+  return v;
+}
+// Sum over the workgroup, in thread 0.
+template <int WAVES> __device__ __forceinline__ double block_sum(double v) {
+  __shared__ double s_wave[WAVES];
+  v = wave_sum(v);
+  if ((threadIdx.x & (kWave - 1)) == 0) s_wave[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double sum = 0.0;
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) sum += s_wave[w];
+  }
+  return sum;
+}
+
+template <typename T>
+__global__ __launch_bounds__(kBlockThreads) void square_sum_kernel(TensorList list, double *__restrict__ partial) {
+  using V = Vec16<T>;
+  double sum = 0.0;
+  for (int chunk = blockIdx.x; chunk < list.chunks; chunk += gridDim.x) {
+    const int t = tensor_of_chunk(list, chunk);
+    const T *src = static_cast<const T *>(list.src[t]);
+    const int offset = static_cast<int>((reinterpret_cast<uint64_t>(src) & 15) / sizeof(T));
+    const V *base = reinterpret_cast<const V *>(src - offset);
+    const int64_t end = offset + list.numel[t];  // in elements from `base`
+    const int64_t first = static_cast<int64_t>(chunk - (t ? list.chunk_end[t - 1] : 0)) * list.chunk_vectors;
+    const int64_t last = min(first + list.chunk_vectors, (end + V::kCount - 1) / V::kCount);
+    for (int64_t i = first + threadIdx.x; i < last; i += kBlockThreads) {
+      if (i * V::kCount >= offset && (i + 1) * V::kCount <= end) {
+        const V x = base[i];
+#pragma unroll
+        for (int q = 0; q < V::kCount; ++q) {
+          const double d = static_cast<double>(x.v[q]);
+          sum += d * d;
+        }
+      } else {
+        const T *e = reinterpret_cast<const T *>(base + i);
+#pragma unroll
+        for (int q = 0; q < V::kCount; ++q) {
+          const int64_t at = i * V::kCount + q;
+          if (at >= offset && at < end) {
+            const double d = static_cast<double>(e[q]);
+            sum += d * d;
+          }
+        }
+      }
+    }
+  }
+  sum = block_sum<kWavesPerBlock>(sum);
+  if (threadIdx.x == 0) partial[blockIdx.x] = sum;
+}
+
+constexpr int kFinishThreads = 1024;
+__global__ __launch_bounds__(kFinishThreads) void norm_finish_kernel(const double *__restrict__ partial, int64_t count,
+                                                                    void *norm, int f64) {
+  double sum = 0.0;
+  for (int64_t i = threadIdx.x; i < count; i += kFinishThreads) sum += partial[i];
+  sum = block_sum<kFinishThreads / kWave>(sum);
+  if (threadIdx.x == 0) {
+    if (f64) *static_cast<double *>(norm) = sqrt(sum);
+    else *static_cast<float *>(norm) = static_cast<float>(sqrt(sum));
+  }
+}
+
+// The norm is rounded once, to the type it is stored in; the scale is formed in 64 bits from it.
+__device__ __forceinline__ double clip_scale(const void *norm, int f64, double max_norm) {
+  const double n = f64 ? *static_cast<const double *>(norm) : static_cast<double>(*static_cast<const float *>(norm));
+  const double scale = max_norm / (n + 1e-6);
+  // (no limit: nothing is scaled, infinities included)
+  return scale > 1.0 || (isinf(max_norm) && isinf(n)) ? 1.0 : scale;
+}
+
+// (products in 32 bits for the types of up to 32, rounded once more for those of 16)
+template <typename T>
+__global__ __launch_bounds__(kBlockThreads) void scale_kernel(TensorList list, const void *norm, int f64, double max_norm) {
+  using A = typename AccOf<T>::type;
+  using V = Vec16<T>;
+  const A scale = static_cast<A>(clip_scale(norm, f64, max_norm));
+  for (int chunk = blockIdx.x; chunk < list.chunks; chunk += gridDim.x) {
+    const int t = tensor_of_chunk(list, chunk);
+    const T *src = static_cast<const T *>(list.src[t]);
+    T *dst = static_cast<T *>(list.dst[t]);
+    if (dst == src && scale == A(1)) continue;  // in place and within the limit: nothing changes
+    const int offset = static_cast<int>((reinterpret_cast<uint64_t>(src) & 15) / sizeof(T));
+    const bool together = ((reinterpret_cast<uint64_t>(src) ^ reinterpret_cast<uint64_t>(dst)) & 15) == 0;
+    const V *base = reinterpret_cast<const V *>(src - offset);
+    T *out = dst - offset;
+    const int64_t end = offset + list.numel[t];
+    const int64_t first = static_cast<int64_t>(chunk - (t ? list.chunk_end[t - 1] : 0)) * list.chunk_vectors;
+    const int64_t last = min(first + list.chunk_vectors, (end + V::kCount - 1) / V::kCount);
+    for (int64_t i = first + threadIdx.x; i < last; i += kBlockThreads) {
+      if (i * V::kCount >= offset && (i + 1) * V::kCount <= end) {
+        V x = base[i];
+#pragma unroll
+        for (int q = 0; q < V::kCount; ++q) x.v[q] = static_cast<T>(static_cast<A>(x.v[q]) * scale);
+        if (together) {
+          reinterpret_cast<V *>(out)[i] = x;
+        } else {
+#pragma unroll
+          for (int q = 0; q < V::kCount; ++q) out[i * V::kCount + q] = x.v[q];
+        }
+      } else {
+        const T *e = reinterpret_cast<const T *>(base + i);
+#pragma unroll
+        for (int q = 0; q < V::kCount; ++q) {
+          const int64_t at = i * V::kCount + q;
+          if (at >= offset && at < end) out[at] = static_cast<T>(static_cast<A>(e[q]) * scale);
+        }
+      }
+    }
+  }
+}
+
+// --------------------------------------------------------------------- norm of the tables' gradient
+// One wavefront per tile of kTile consecutive sorted positions and column block of up to 64 vectors; each of
+// its lane groups (one 16-byte vector of the row per lane) walks a run of consecutive positions, adding rows of
+// one segment and squaring the sum where the segment ends.  No sum over lanes is needed before the very end:
+// a lane squares its own columns.  A segment that crosses the ends of runs leaves partial sums in LDS, which lane
+// group 0 joins; one that crosses the ends of tiles leaves partial rows (row 2 * tile: what ends in the
+// tile or runs through it, row 2 * tile + 1: what begins in it and goes on), which the next launch joins from
+// the tile where the segment begins.
+constexpr int kTile = 256;
+
+template <typename T, int VEC, bool WEIGHTED>
+__global__ __launch_bounds__(kBlockThreads) void table_norm_tiles_kernel(
+    const T *__restrict__ grad, const T *__restrict__ psw, const int32_t *__restrict__ positions_sorted,
+    const int32_t *__restrict__ grad_rows, const int32_t *__restrict__ segment_ids, int64_t n, int D,
+    int64_t num_tiles, typename AccOf<T>::type *__restrict__ partial_rows, double *__restrict__ tile_sums) {
+  using V = RowVec<T, VEC>;
+  using A = typename V::A;
+  using R = typename V::R;
+  constexpr int kAhead = 8;
+  __shared__ int32_t s_segment[kWavesPerBlock][kTile];
+  __shared__ int32_t s_row[kWavesPerBlock][kTile];
+  __shared__ A s_weight[WEIGHTED ? kWavesPerBlock : 1][WEIGHTED ? kTile : 1];
+  __shared__ A s_head[kWavesPerBlock][kWave][VEC];
+  __shared__ A s_tail[kWavesPerBlock][kWave][VEC];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = threadIdx.x >> 6;
+  const int64_t tile = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + wave;
+  if (tile >= num_tiles) return;
+  const int64_t p0 = tile * kTile;
+  const int len = static_cast<int>(min(n - p0, static_cast<int64_t>(kTile)));
+#pragma unroll
+  for (int q = 0; q < kTile / kWave; ++q) {
+    const int i = q * kWave + lane;
+    const int64_t p = p0 + min(i, len - 1);
+    const int pos = positions_sorted[p];
+    s_segment[wave][i] = segment_ids[p];
+    s_row[wave][i] = grad_rows[pos];
+    if constexpr (WEIGHTED) s_weight[wave][i] = to_acc(psw[pos]);
+  }
+  wave_sync();
+  const bool open_before = p0 > 0 && segment_ids[max(p0 - 1, int64_t{0})] == s_segment[wave][0];
+  const bool open_after = p0 + len < n && segment_ids[min(p0 + len, n - 1)] == s_segment[wave][len - 1];
+
+  const int vectors = D / VEC - blockIdx.y * kWave;      // of the columns from this block's first on
+  const int chunks = vectors < kWave ? vectors : kWave;
+  const int groups = kWave / chunks;
+  const int run = (len + groups - 1) / groups;
+  const int r = lane / chunks;
+  const int c = lane - r * chunks;
+  const int64_t col = (static_cast<int64_t>(blockIdx.y) * kWave + c) * VEC;
+  const int begin = min(r * run, len), end = min(begin + run, len);
+  auto opens = [&](int b) { return b == 0 ? open_before : s_segment[wave][b - 1] == s_segment[wave][b]; };
+  auto goes_on = [&](int e) { return e == len ? open_after : s_segment[wave][e - 1] == s_segment[wave][e]; };
+
+  double squares = 0.0;
+  if (r < groups && begin < end) {
+    V G;
+    G.zero();
+    bool head = opens(begin);  // the segment being added began before this run
+    int current = s_segment[wave][begin];
+    auto close = [&]() {
+      if (head) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) s_head[wave][lane][k] = G.v[k];
+        head = false;
+      } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) squares += static_cast<double>(G.v[k]) * static_cast<double>(G.v[k]);
+      }
+      G.zero();
+    };
+    for (int i0 = begin; i0 < end; i0 += kAhead) {
+      R raw[kAhead];
+#pragma unroll
+      for (int q = 0; q < kAhead; ++q) {
+        const int i = min(i0 + q, end - 1);  // clamped, not predicated: no branch per load
+        raw[q] = V::load_raw(grad + static_cast<int64_t>(s_row[wave][i]) * D + col);
+      }
+#pragma unroll
+      for (int q = 0; q < kAhead; ++q) {
+        const int i = i0 + q;
+        if (i >= end) break;
+        const int segment = s_segment[wave][i];
+        if (segment != current) {
+          close();
+          current = segment;
+        }
+        V x;
+        x.unpack(raw[q]);
+        A w = A(1);
+        if constexpr (WEIGHTED) w = s_weight[wave][i];
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) G.v[k] += WEIGHTED ? x.v[k] * w : x.v[k];
+      }
+    }
+    if (goes_on(end) && !head) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) s_tail[wave][lane][k] = G.v[k];
+    } else {
+      close();  // (a segment that runs through the whole run is kept like one that ends in it)
+    }
+  }
+  wave_sync();
+  if (r == 0) {
+    V open;
+    open.zero();
+    bool from_before = open_before;
+    A *rows = partial_rows + 2 * tile * D + col;
+    for (int g = 0; g < groups; ++g) {
+      const int b = min(g * run, len), e = min(b + run, len);
+      if (b >= e) break;
+      const bool through = opens(b) && goes_on(e) && s_segment[wave][b] == s_segment[wave][e - 1];
+      if (opens(b)) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) open.v[k] += s_head[wave][g * chunks + c][k];
+        if (through) continue;
+        if (from_before) {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) rows[k] = open.v[k];
+          from_before = false;
+        } else {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) squares += static_cast<double>(open.v[k]) * static_cast<double>(open.v[k]);
+        }
+        open.zero();
+      }
+      if (goes_on(e)) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) open.v[k] = s_tail[wave][g * chunks + c][k];
+      }
+    }
+    if (open_after) {
+      if (!from_before) rows += D;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) rows[k] = open.v[k];
+    }
+  }
+  squares = wave_sum(squares);
+  if (lane == 0) tile_sums[tile * gridDim.y + blockIdx.y] = squares;
+}
+
+// The segments that cross tiles: a wavefront per tile, working where one begins and goes on, adds the
+// partial rows of the tiles up to its end; a workgroup's wavefronts then add up their tiles' squares.
+template <typename T, int VEC>
+__global__ __launch_bounds__(kBlockThreads) void table_norm_join_kernel(
+    const int32_t *__restrict__ segment_ids, const int32_t *__restrict__ segment_starts, int64_t n, int D,
+    int64_t num_tiles, const typename AccOf<T>::type *__restrict__ partial_rows,
+    const double *__restrict__ tile_sums, int column_blocks, double *__restrict__ partial) {
+  using A = typename AccOf<T>::type;
+  const int lane = threadIdx.x & (kWave - 1);
+  double squares = 0.0;  // (of this lane)
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kWavesPerBlock;
+  for (int64_t tile = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + (threadIdx.x >> 6); tile < num_tiles;
+       tile += stride) {
+    for (int b = lane; b < column_blocks; b += kWave) squares += tile_sums[tile * column_blocks + b];
+    const int64_t next = (tile + 1) * kTile;
+    if (next >= n) continue;
+    const int segment = segment_ids[next - 1];
+    if (segment_ids[next] != segment) continue;
+    if (segment_starts[segment] < tile * kTile) continue;  // it began in an earlier tile, which joins it
+    const int64_t last = (static_cast<int64_t>(segment_starts[segment + 1]) - 1) / kTile;
+    for (int v0 = 0; v0 < D / VEC; v0 += kWave) {
+      const int chunks = min(kWave, D / VEC - v0);
+      const int groups = kWave / chunks;
+      const int r = lane / chunks;
+      const int c = lane - r * chunks;
+      const int64_t col = static_cast<int64_t>(v0 + c) * VEC;
+      A sum[VEC];
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) sum[k] = A(0);
+      if (r < groups) {
+        for (int64_t t = tile + r; t <= last; t += groups) {
+          const A *row = partial_rows + (2 * t + (t == tile ? 1 : 0)) * D + col;
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) sum[k] += row[k];
+        }
+      }
+      for (int g = 1; g < groups; ++g) {
+        const int from = min(lane + g * chunks, kWave - 1);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          const A o = shfl_idx(sum[k], from);
+          if (r == 0) sum[k] += o;
+        }
+      }
+      if (r == 0) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) squares += static_cast<double>(sum[k]) * static_cast<double>(sum[k]);
+      }
+    }
+  }
+  squares = block_sum<kWavesPerBlock>(squares);
+  if (threadIdx.x == 0) partial[blockIdx.x] = squares;
+}
+
+// ------------------------------------------------------------------------------------------ host
+constexpr int kMaxBlocks = 256 * 8;   // of a launch over a list: eight workgroups per compute unit
+constexpr int kJoinBlocks = 1024;
+
+size_t size_of(int32_t dtype) { return dtype == TBE_DTYPE_F64 ? 8 : dtype == TBE_DTYPE_F32 ? 4 : 2; }
+
+// A list of one type, in pieces of kListTensors tensors.  f(list) is called for every piece.
+template <typename F>
+void for_lists(const void *const *src, void *const *dst, const int64_t *numel, const int32_t *dtypes, int32_t count,
+               int32_t dtype, int chunk_vectors, F &&f) {
+  TensorList list;
+  list.count = 0;
+  list.chunks = 0;
+  list.chunk_vectors = chunk_vectors;
+  for (int32_t i = 0; i < count; ++i) {
+    if (dtypes[i] != dtype || numel[i] == 0) continue;
+    const uint64_t offset = reinterpret_cast<uint64_t>(src[i]) & 15;
+    const int64_t chunks = ceil_div(ceil_div(static_cast<int64_t>(offset + numel[i] * size_of(dtype)), 16), chunk_vectors);
+    if (list.count == kListTensors || list.chunks + chunks > INT32_MAX / 2) {
+      f(list);
+      list.count = list.chunks = 0;
+    }
+    list.src[list.count] = src[i];
+    list.dst[list.count] = dst ? dst[i] : nullptr;
+    list.numel[list.count] = numel[i];
+    list.chunks += static_cast<int32_t>(chunks);
+    list.chunk_end[list.count++] = list.chunks;
+  }
+  if (list.count) f(list);
+}
+
+// 16 KB a chunk
+constexpr int kChunkVectors = 1024;
+
+struct ListCall {
+  const void *const *gradients;
+  void *const *outputs;
+  const int64_t *numels;
+  const int32_t *dtypes;
+  int32_t count;
+};
+
+int check_list(const char *name, const ListCall &c, bool outputs) {
+  TBE_REQUIRE(c.count >= 0, "%s: num_tensors must not be negative", name);
+  TBE_REQUIRE(c.count == 0 || (c.gradients && c.numels && c.dtypes && (c.outputs || !outputs)),
+              "%s: null pointer argument", name);
+  for (int32_t i = 0; i < c.count; ++i) {
+    TBE_REQUIRE(c.dtypes[i] >= TBE_DTYPE_F32 && c.dtypes[i] <= TBE_DTYPE_BF16, "%s: bad dtype %d", name, c.dtypes[i]);
+    const uint64_t size = size_of(c.dtypes[i]);
+    TBE_REQUIRE(c.numels[i] >= 0 && c.numels[i] <= (int64_t{1} << 40), "%s: element count of tensor %d out of range", name, i);
+    if (c.numels[i] == 0) continue;
+    TBE_REQUIRE(c.gradients[i] && (!outputs || c.outputs[i]), "%s: null pointer argument", name);
+    TBE_REQUIRE(reinterpret_cast<uint64_t>(c.gradients[i]) % size == 0 &&
+                    (!outputs || reinterpret_cast<uint64_t>(c.outputs[i]) % size == 0),
+                "%s: misaligned pointer of tensor %d", name, i);
+  }
+  return TBE_OK;
+}
+
+// An output may be its own gradient; apart from that no output may share memory with another output or with
+// another tensor's gradient: two workgroups would write there, or one read what another has scaled.
+int check_overlap(const char *name, const ListCall &c) {
+  struct Range {
+    uint64_t begin, end;
+    int32_t tensor;
+    bool written;
+  };
+  try {
+    std::vector<Range> ranges;
+    ranges.reserve(2 * static_cast<size_t>(c.count));
+    for (int32_t i = 0; i < c.count; ++i) {
+      if (c.numels[i] == 0) continue;
+      const uint64_t bytes = static_cast<uint64_t>(c.numels[i]) * size_of(c.dtypes[i]);
+      const uint64_t out = reinterpret_cast<uint64_t>(c.outputs[i]), in = reinterpret_cast<uint64_t>(c.gradients[i]);
+      ranges.push_back(Range{out, out + bytes, i, true});
+      if (in != out) ranges.push_back(Range{in, in + bytes, i, false});
+    }
+    std::sort(ranges.begin(), ranges.end(), [](const Range &a, const Range &b) { return a.begin < b.begin; });
+    // the furthest ends so far, of what is written and of what is only read
+    uint64_t written_end = 0, read_end = 0;
+    for (const Range &r : ranges) {
+      TBE_REQUIRE(r.begin >= written_end && (!r.written || r.begin >= read_end),
+                  "%s: tensor %d shares memory with another one of the list", name, r.tensor);
+      (r.written ? written_end : read_end) = std::max(r.written ? written_end : read_end, r.end);
+    }
+  } catch (const std::bad_alloc &) {
+    return fail(TBE_ERR_INVALID, "%s: out of host memory", name);
+  }
+  return TBE_OK;
+}
+
+unsigned list_grid(const TensorList &list) { return static_cast<unsigned>(std::min(list.chunks, kMaxBlocks)); }
+
+constexpr int32_t kDtypes[] = {TBE_DTYPE_F32, TBE_DTYPE_F16, TBE_DTYPE_BF16, TBE_DTYPE_F64};
+
+// (every type of a list starts pieces of its own, so there are at most this many)
+int64_t max_pieces(int32_t count) { return count / kListTensors + 4; }
+
+void launch_norm(const ListCall &c, void *workspace, void *norm, int32_t norm_dtype, hipStream_t s) {
+  double *partial = static_cast<double *>(workspace);
+  int64_t used = 0;
+  for (const int32_t dtype : kDtypes) {
+    for_lists(c.gradients, nullptr, c.numels, c.dtypes, c.count, dtype, kChunkVectors, [&](const TensorList &list) {
+      const dim3 grid(list_grid(list)), block(kBlockThreads);
+      switch (dtype) {
+        case TBE_DTYPE_F32: TBE_LAUNCH("gradient_squares", s, square_sum_kernel<float>, grid, block, list, partial + used); break;
+        case TBE_DTYPE_F16: TBE_LAUNCH("gradient_squares", s, square_sum_kernel<_Float16>, grid, block, list, partial + used); break;
+        case TBE_DTYPE_BF16: TBE_LAUNCH("gradient_squares", s, square_sum_kernel<__bf16>, grid, block, list, partial + used); break;
+        default: TBE_LAUNCH("gradient_squares", s, square_sum_kernel<double>, grid, block, list, partial + used); break;
+      }
+      used += grid.x;
+    });
+  }
+  TBE_LAUNCH("gradient_norm", s, norm_finish_kernel, dim3(1), dim3(kFinishThreads), partial, used, norm,
+             norm_dtype == TBE_DTYPE_F64 ? 1 : 0);
+}
+
+void launch_scale(const ListCall &c, double max_norm, const void *norm, int32_t norm_dtype, hipStream_t s) {
+  const int f64 = norm_dtype == TBE_DTYPE_F64 ? 1 : 0;
+  for (const int32_t dtype : kDtypes) {
+    for_lists(c.gradients, c.outputs, c.numels, c.dtypes, c.count, dtype, kChunkVectors, [&](const TensorList &list) {
+      const dim3 grid(list_grid(list)), block(kBlockThreads);
+      switch (dtype) {
+        case TBE_DTYPE_F32: TBE_LAUNCH("gradient_scale", s, scale_kernel<float>, grid, block, list, norm, f64, max_norm); break;
+        case TBE_DTYPE_F16: TBE_LAUNCH("gradient_scale", s, scale_kernel<_Float16>, grid, block, list, norm, f64, max_norm); break;
+        case TBE_DTYPE_BF16: TBE_LAUNCH("gradient_scale", s, scale_kernel<__bf16>, grid, block, list, norm, f64, max_norm); break;
+        default: TBE_LAUNCH("gradient_scale", s, scale_kernel<double>, grid, block, list, norm, f64, max_norm); break;
+      }
+    });
+  }
+}
+
+int check_norm(const char *name, const void *norm, int32_t norm_dtype) {
+  TBE_REQUIRE(norm, "%s: norm is null", name);
+  TBE_REQUIRE(norm_dtype == TBE_DTYPE_F32 || norm_dtype == TBE_DTYPE_F64, "%s: the norm is F32 or F64 (got %d)", name, norm_dtype);
+  return TBE_OK;
+}
+
+int check_workspace(const char *name, int32_t count, const void *workspace, uint64_t bytes) {
+  const uint64_t need = tbe_gradient_norm_workspace_bytes(count);
+  if (!workspace || bytes < need)
+    return fail(TBE_ERR_WORKSPACE, "%s: workspace of %llu bytes needed, %llu given", name, (unsigned long long)need,
+                (unsigned long long)bytes);
+  return TBE_OK;
+}
+
+struct TableCall {
+  const void *grad, *psw;
+  const int32_t *positions_sorted, *grad_rows, *segment_ids, *segment_starts;
+  int64_t n;
+  int32_t D;
+  void *partial_rows;
+  double *tile_sums, *partial;
+  hipStream_t stream;
+};
+
+template <typename T, int VEC> unsigned launch_table(const TableCall &c, int64_t tiles, int column_blocks) {
+  using A = typename AccOf<T>::type;
+  const dim3 grid(static_cast<unsigned>(ceil_div(tiles, kWavesPerBlock)), column_blocks), block(kBlockThreads);
+  const T *grad = static_cast<const T *>(c.grad), *psw = static_cast<const T *>(c.psw);
+  A *rows = static_cast<A *>(c.partial_rows);
+  if (psw)
+    TBE_LAUNCH("table_norm_tiles", c.stream, (table_norm_tiles_kernel<T, VEC, true>), grid, block, grad, psw,
+               c.positions_sorted, c.grad_rows, c.segment_ids, c.n, c.D, tiles, rows, c.tile_sums);
+  else
+    TBE_LAUNCH("table_norm_tiles", c.stream, (table_norm_tiles_kernel<T, VEC, false>), grid, block, grad, psw,
+               c.positions_sorted, c.grad_rows, c.segment_ids, c.n, c.D, tiles, rows, c.tile_sums);
+  const unsigned join = static_cast<unsigned>(std::min<int64_t>(ceil_div(tiles, kWavesPerBlock), kJoinBlocks));
+  TBE_LAUNCH("table_norm_join", c.stream, (table_norm_join_kernel<T, VEC>), dim3(join), block, c.segment_ids,
+             c.segment_starts, c.n, c.D, tiles, rows, c.tile_sums, column_blocks, c.partial);
+  return join;
+}
+
+}  // namespace
+}  // namespace tbe
+
+extern "C" uint64_t tbe_gradient_norm_workspace_bytes(int32_t num_tensors) {
+  if (num_tensors < 0) return 0;
+  return static_cast<uint64_t>(tbe::max_pieces(num_tensors)) * tbe::kMaxBlocks * sizeof(double);
+}
+
+extern "C" int tbe_gradient_norm(const void *const *gradients, const int64_t *numels, const int32_t *dtypes,
+                                 int32_t num_tensors, void *norm, int32_t norm_dtype, void *workspace,
+                                 uint64_t workspace_bytes, void *stream) {
+  using namespace tbe;
+  const char *name = "tbe_gradient_norm";
+  const ListCall c{gradients, nullptr, numels, dtypes, num_tensors};
+  if (int rc = check_list(name, c, false)) return rc;
+  if (int rc = check_norm(name, norm, norm_dtype)) return rc;
+  if (int rc = check_workspace(name, num_tensors, workspace, workspace_bytes)) return rc;
+  launch_norm(c, workspace, norm, norm_dtype, static_cast<hipStream_t>(stream));
+  return check_launch(name);
+}
+
+extern "C" int tbe_scale_gradients(const void *const *gradients, void *const *outputs, const int64_t *numels,
+                                   const int32_t *dtypes, int32_t num_tensors, double max_norm, const void *norm,
+                                   int32_t norm_dtype, void *stream) {
+  using namespace tbe;
+  const char *name = "tbe_scale_gradients";
+  const ListCall c{gradients, outputs, numels, dtypes, num_tensors};
+  if (int rc = check_list(name, c, true)) return rc;
+  if (int rc = check_norm(name, norm, norm_dtype)) return rc;
+  TBE_REQUIRE(max_norm >= 0.0, "%s: max_norm must not be negative", name);
+  if (int rc = check_overlap(name, c)) return rc;
+  launch_scale(c, max_norm, norm, norm_dtype, static_cast<hipStream_t>(stream));
+  return check_launch(name);
+}
+
+extern "C" int tbe_clip_gradients(const void *const *gradients, void *const *outputs, const int64_t *numels,
+                                  const int32_t *dtypes, int32_t num_tensors, double max_norm, void *norm,
+                                  int32_t norm_dtype, void *workspace, uint64_t workspace_bytes, void *stream) {
+  using namespace tbe;
+  const char *name = "tbe_clip_gradients";
+  const ListCall c{gradients, outputs, numels, dtypes, num_tensors};
+  if (int rc = check_list(name, c, true)) return rc;
+  if (int rc = check_norm(name, norm, norm_dtype)) return rc;
+  TBE_REQUIRE(max_norm >= 0.0, "%s: max_norm must not be negative", name);
+  if (int rc = check_workspace(name, num_tensors, workspace, workspace_bytes)) return rc;
+  if (int rc = check_overlap(name, c)) return rc;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  launch_norm(c, workspace, norm, norm_dtype, s);
+  launch_scale(c, max_norm, norm, norm_dtype, s);
+  return check_launch(name);
+}
+
+extern "C" int tbe_table_gradient_norm(const void *grad_output, int32_t dtype, int32_t D, int32_t T, int32_t B,
+                                       int64_t num_indices, const void *per_sample_weights, void *workspace,
+                                       uint64_t workspace_bytes, void *norm, int32_t norm_dtype, void *stream) {
+  using namespace tbe;
+  const char *name = "tbe_table_gradient_norm";
+  TBE_REQUIRE(T > 0 && B > 0, "%s: T and B must be positive (got %d, %d)", name, T, B);
+  TBE_REQUIRE(D > 0 && D % 4 == 0, "%s: D must be a positive multiple of 4 (got %d)", name, D);
+  TBE_REQUIRE(dtype >= TBE_DTYPE_F32 && dtype <= TBE_DTYPE_F64, "%s: bad dtype %d", name, dtype);
+  TBE_REQUIRE(num_indices >= 0 && num_indices < INT32_MAX, "%s: num_indices out of range", name);
+  TBE_REQUIRE(static_cast<int64_t>(T) * B < INT32_MAX, "%s: T*B out of range", name);
+  TBE_REQUIRE(grad_output, "%s: null pointer argument", name);
+  if (int rc = check_norm(name, norm, norm_dtype)) return rc;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int f64 = norm_dtype == TBE_DTYPE_F64 ? 1 : 0;
+  if (num_indices == 0) {
+    TBE_LAUNCH("gradient_norm", s, norm_finish_kernel, dim3(1), dim3(kFinishThreads), nullptr, int64_t{0}, norm, f64);
+    return check_launch(name);
+  }
+  tbe_workspace_layout_t l;
+  backward_layout(num_indices, D, dtype, T, &l);
+  if (!workspace || workspace_bytes < l.total_bytes)
+    return fail(TBE_ERR_WORKSPACE, "%s: workspace of %llu bytes needed, %llu given", name,
+                (unsigned long long)l.total_bytes, (unsigned long long)workspace_bytes);
+  const RowGeometry g = row_geometry(dtype, D);
+  const int64_t tiles = ceil_div(num_indices, kTile);
+  const int64_t column_blocks = ceil_div(g.chunks, kWave);
+  // The update's queues and partial rows are not in use between a plan and its update: the tiles' sums go to the
+  // chunk records' room, the partial rows (two per kTile positions, like the update's) to their own.
+  static_assert(kTile == kChunkLen, "two partial rows per tile fit the update's");
+  const uint64_t sums = static_cast<uint64_t>(tiles * column_blocks + kJoinBlocks) * sizeof(double);
+  if (sums > l.partial_sums - l.chunk_segments || column_blocks > 65535)
+    return fail(TBE_ERR_UNSUPPORTED, "%s: rows of %d elements are too wide", name, D);
+  char *ws = static_cast<char *>(workspace);
+  TableCall c;
+  c.grad = grad_output;
+  c.psw = per_sample_weights;
+  c.positions_sorted = reinterpret_cast<const int32_t *>(ws + l.positions_sorted);
+  c.grad_rows = reinterpret_cast<const int32_t *>(ws + l.grad_rows);
+  c.segment_ids = reinterpret_cast<const int32_t *>(ws + l.segment_ids);
+  c.segment_starts = reinterpret_cast<const int32_t *>(ws + l.segment_starts);
+  c.n = num_indices;
+  c.D = D;
+  c.partial_rows = ws + l.partial_sums;
+  c.partial = reinterpret_cast<double *>(ws + l.chunk_segments);
+  c.tile_sums = c.partial + kJoinBlocks;
+  c.stream = s;
+  unsigned parts;
+  switch (dtype) {
+    case TBE_DTYPE_F32: parts = launch_table<float, 4>(c, tiles, static_cast<int>(column_blocks)); break;
+    case TBE_DTYPE_F16:
+      parts = g.vec == 8 ? launch_table<__half, 8>(c, tiles, static_cast<int>(column_blocks))
+                         : launch_table<__half, 4>(c, tiles, static_cast<int>(column_blocks));
+      break;
+    default: parts = launch_table<double, 2>(c, tiles, static_cast<int>(column_blocks)); break;
+  }
+  TBE_LAUNCH("gradient_norm", s, norm_finish_kernel, dim3(1), dim3(kFinishThreads), c.partial,
+             static_cast<int64_t>(parts), norm, f64);
+  return check_launch(name);
+}

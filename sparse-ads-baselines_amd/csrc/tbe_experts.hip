@@ -23,7 +23,7 @@ namespace {
 // ranks a tile's pairs with wavefront ballots (all lanes of one expert are found with one ballot per bit
 // of the expert's number) and places them.  Pairs inside a tile are numbered (wavefront, item, lane),
 // which the ranking keeps, so the order is stable.
-constexpr int kMaxExperts = 4095;   // and one bin more for the dropped pairs
+constexpr int kMaxExperts = TBE_MAX_EXPERTS;  // and one bin more for the dropped pairs
 constexpr int kTileWaves = 4, kTileItems = 8;
 constexpr int kPlanTile = kTileWaves * kWave * kTileItems;
 constexpr int kSmallWaves = 16, kSmallItems = 8;
@@ -262,7 +262,8 @@ __global__ __launch_bounds__(kBlockThreads) void expert_combine_kernel(
 }
 
 // GROUP lanes per token (a workgroup per token for GROUP = 256): the token's gradient row is read once per
-// kChoices choices, every chosen row is read and its gradient written once.
+// kChoices choices, every chosen row is read and its gradient written once.  Without grad_weights the rows are
+// not read, without grad_rows nothing is written to them.
 template <typename T, typename W, int VEC, int GROUP>
 __global__ __launch_bounds__(kBlockThreads) void expert_combine_backward_kernel(
     const T *__restrict__ grad, int64_t grad_stride, const T *__restrict__ rows, int64_t row_stride,
@@ -298,16 +299,18 @@ __global__ __launch_bounds__(kBlockThreads) void expert_combine_backward_kernel(
         if (place[j] < 0) continue;
         const bool keep = place[j] < kept;
         P o;
-        if (keep) {
+        if (keep && grad_weights) {
           const P v = *reinterpret_cast<const P *>(rows + place[j] * row_stride + static_cast<int64_t>(col) * VEC);
 #pragma unroll
           for (int q = 0; q < VEC; ++q) dot[j] += static_cast<A>(v.v[q]) * static_cast<A>(gv.v[q]);
         }
+        if (!grad_rows) continue;
 #pragma unroll
         for (int q = 0; q < VEC; ++q) o.v[q] = keep ? static_cast<T>(w[j] * static_cast<A>(gv.v[q])) : T(0);
         *reinterpret_cast<P *>(grad_rows + (static_cast<int64_t>(place[j]) * vectors + col) * VEC) = o;
       }
     }
+    if (!grad_weights) continue;
 #pragma unroll
     for (int j = 0; j < kChoices; ++j) {
 #pragma unroll
@@ -602,7 +605,8 @@ extern "C" int tbe_expert_combine_backward(const void *grad_output, int64_t grad
   TBE_REQUIRE(weights_dtype == TBE_DTYPE_F32 || weights_dtype == dtype,
               "%s: weights must be fp32 or of the rows' type", name);
   if (num_tokens == 0) return TBE_OK;
-  TBE_REQUIRE(grad_output && rows && places && expert_offsets && weights && grad_rows && grad_weights,
+  TBE_REQUIRE(grad_output && places && expert_offsets && weights && (rows || !grad_weights) &&
+                  (grad_rows || grad_weights),
               "%s: null pointer argument", name);
   const uint64_t size = element_size(dtype);
   const int bytes = vector_bytes(D * size | row_stride * size | grad_stride * size | address(rows) |

@@ -19,6 +19,9 @@ from torch import nn
 
 import table_batched_embeddings
 import table_batched_embeddings_cache
+import tbe_native
+from table_batched_embeddings_clip import (  # noqa: F401  (extensions, part of this module's surface)
+    clip_grad_norm_, clip_gradients, clip_table_gradient, gradient_norm)
 from table_batched_embeddings_experts import (  # noqa: F401  (extensions, part of this module's surface)
     ExpertRouting, expert_combine, expert_dispatch, expert_plan)
 
@@ -63,7 +66,11 @@ class LookupFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, weights, table_offsets, indices, offsets, per_sample_weights, optimizer,
-                optimizer_state, learning_rate, eps, stochastic_rounding):
+                optimizer_state, learning_rate, eps, stochastic_rounding, clip=None):
+        if clip is not None and ctx.needs_input_grad[4]:
+            # (their gradient is formed inside the table update, from the gradient that was clipped for the tables)
+            raise RuntimeError("clip_gradient does not go with per-sample weights that need a gradient")
+        ctx.clip = clip
         ctx.optimizer = optimizer
         ctx.learning_rate = learning_rate
         ctx.eps = eps
@@ -76,7 +83,7 @@ class LookupFunction(torch.autograd.Function):
         # the slots it leaves, so the step time is unchanged.  Off unless a caller opts in.
         ctx.plan = None
         if (LookupFunction.plan_ahead and any(ctx.needs_input_grad)
-                and optimizer != Optimizer.APPROX_ROWWISE_ADAGRAD):
+                and optimizer != Optimizer.APPROX_ROWWISE_ADAGRAD and clip is None):
             ctx.plan = table_batched_embeddings.plan_backward(weights, table_offsets, indices, offsets)
         return extension.forward(
             weights, table_offsets, indices, offsets, per_sample_weights, L_max,
@@ -89,9 +96,11 @@ class LookupFunction(torch.autograd.Function):
         assert ctx.optimizer in (Optimizer.SGD, Optimizer.APPROX_ROWWISE_ADAGRAD,
                                  Optimizer.EXACT_ROWWISE_ADAGRAD)
         plan, ctx.plan = ctx.plan, None
-        if plan is not None:
+        if ctx.clip is not None:
+            ctx.clip.update(ctx, grad_output, L_max)
+            grad_per_sample_weight = None
+        elif plan is not None:
             assert ctx.optimizer != Optimizer.SGD or per_sample_weights is None
-            import tbe_native
             code = tbe_native.OPT_SGD if ctx.optimizer == Optimizer.SGD else tbe_native.OPT_ROWWISE_ADAGRAD
             grad_per_sample_weight = plan.apply(code, grad_output, weights, per_sample_weights, optimizer_state,
                                                 ctx.learning_rate, ctx.eps, ctx.stochastic_rounding)
@@ -116,7 +125,34 @@ class LookupFunction(torch.autograd.Function):
                 torch.empty((2, 0), dtype=torch.int64, device=weights.device),
                 torch.empty((0,), dtype=weights.dtype, device=weights.device),
                 size=tuple(weights.shape))
-        return (empty_grad, None, None, None, grad_per_sample_weight, None, None, None, None, None)
+        return (empty_grad, None, None, None, grad_per_sample_weight, None, None, None, None, None, None)
+
+
+class TableGradientClip:
+    """Clips the exact gradient of a module's tables to a norm, inside backward, before the fused update.
+    `norm` is the norm that the last backward's gradient had (a 0-dim tensor on the device), None before the
+    first."""
+
+    def __init__(self, max_norm):
+        self.max_norm = float(max_norm)
+        self.norm = None
+        if not self.max_norm >= 0.0:
+            raise RuntimeError("max_norm must not be negative")
+
+    def update(self, ctx, grad_output, L_max):
+        (weights, table_offsets, indices, offsets, per_sample_weights, optimizer_state) = ctx.saved_tensors
+        if ctx.optimizer == Optimizer.APPROX_ROWWISE_ADAGRAD:
+            # (the per-lookup update makes its own plan)
+            grad_output, self.norm = clip_table_gradient(grad_output, weights, table_offsets, indices, offsets,
+                                                         self.max_norm, per_sample_weights)
+            extension.backward_approx_adagrad(
+                grad_output, weights, table_offsets, indices, offsets, per_sample_weights, optimizer_state,
+                ctx.learning_rate, ctx.eps, L_max, ctx.stochastic_rounding, 1)
+            return
+        code = tbe_native.OPT_SGD if ctx.optimizer == Optimizer.SGD else tbe_native.OPT_ROWWISE_ADAGRAD
+        self.norm = tbe_native.compiled().backward_clipped(
+            code, grad_output, weights, table_offsets, indices, offsets, per_sample_weights, optimizer_state,
+            ctx.learning_rate, ctx.eps or 0.0, ctx.stochastic_rounding, self.max_norm)
 
 
 class CachedLookupFunction(torch.autograd.Function):
@@ -235,6 +271,19 @@ class TableBatchedEmbeddingBags(_CacheFronted, nn.Module):
         self.eps = eps
         self.stochastic_rounding = stochastic_rounding
 
+    gradient_clip = None  # set by clip_gradient()
+
+    def clip_gradient(self, max_norm):
+        """From the next forward on, every backward clips the tables' exact gradient (one row per distinct
+        index, the sum over its lookups) to max_norm before the update; None turns it off.  Returns the
+        TableGradientClip, whose `norm` is the last backward's.  The norm is this module's own: a norm over the
+        whole model is not known yet when the tables are updated.  Not for tables behind the row cache, nor with
+        per-sample weights that need a gradient."""
+        if self.row_cache is not None:
+            raise RuntimeError("clip_gradient is not served behind the row cache (EmbeddingLocation.HOST_CACHED)")
+        self.gradient_clip = None if max_norm is None else TableGradientClip(max_norm)
+        return self.gradient_clip
+
     def cache_table_rows(self):
         """First row of each table, as the row cache's calls take it."""
         return self.table_offsets
@@ -268,7 +317,7 @@ class TableBatchedEmbeddingBags(_CacheFronted, nn.Module):
         return LookupFunction.apply(
             self.embedding_weights, self.table_offsets, sharded_sparse_features, sharded_offsets,
             per_sample_weights, self.optimizer, self.optimizer_state, self.learning_rate, self.eps,
-            self.stochastic_rounding)
+            self.stochastic_rounding, self.gradient_clip)
 
 
 class MixedDimLookupFunction(torch.autograd.Function):

@@ -21,6 +21,7 @@ _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
 _u64 = ctypes.c_uint64
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 
 
 class WorkspaceLayout(ctypes.Structure):
@@ -152,6 +153,11 @@ SIGNATURES = {
                                           _vp]),
     "tbe_expert_combine_backward": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i32, _i64, _i32, _i32, _i64, _c_i32p,
                                                    _c_i32p, _vp, _i32, _vp, _vp, _vp]),
+    "tbe_gradient_norm_workspace_bytes": (_u64, [_i32]),
+    "tbe_gradient_norm": (ctypes.c_int, [_vp, _vp, _vp, _i32, _vp, _i32, _vp, _u64, _vp]),
+    "tbe_scale_gradients": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _f64, _vp, _i32, _vp]),
+    "tbe_clip_gradients": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i32, _f64, _vp, _i32, _vp, _u64, _vp]),
+    "tbe_table_gradient_norm": (ctypes.c_int, [_vp, _i32, _i32, _i32, _i32, _i64, _vp, _vp, _u64, _vp, _i32, _vp]),
     "tbe_host_mapped_alloc": (ctypes.c_int, [_u64, ctypes.POINTER(_vp), ctypes.POINTER(_vp)]),
     "tbe_host_mapped_free": (ctypes.c_int, [_vp]),
     "tbe_managed_alloc": (ctypes.c_int, [_u64, _i32, ctypes.POINTER(_vp)]),
@@ -184,6 +190,26 @@ def load():
         fn.argtypes = argtypes
     _lib = lib
     return lib
+
+
+_compiled = None
+
+
+def compiled():
+    """The pybind11 module over the library (table_batched_embeddings_cpp): expert routing and gradient
+    clipping are reached through it.  Raises if it is absent."""
+    global _compiled
+    if _compiled is None:
+        try:
+            import torch  # noqa: F401  (before the library, see load())
+            import table_batched_embeddings_cpp
+        except ImportError as e:
+            raise RuntimeError("table_batched_embeddings_cpp does not load (%s): build it with `python %s`; there is "
+                               "no fallback path" % (e, os.path.join(_HERE, "build.py"))) from e
+        if table_batched_embeddings_cpp.abi_version() != ABI_VERSION:
+            raise RuntimeError("table_batched_embeddings_cpp was built for another library")
+        _compiled = table_batched_embeddings_cpp
+    return _compiled
 
 
 def check(code):

@@ -243,7 +243,7 @@ def test_rows_beyond_32_bit_offsets():
     assert torch.equal(y[:, -1], (x[:, 0].float() * 0.5).to(BF16)) and torch.equal(y[:, 0], y[:, -1])
     del x
     g = torch.ones(tokens, D, device=DEV, dtype=BF16)
-    grad_rows, grad_weights = experts_mod._combine_backward(g, rows, routing.places, routing.expert_offsets, w)
+    grad_rows, grad_weights = experts_mod.compiled().expert_combine_backward(g, rows, routing.places, routing.expert_offsets, w)
     assert bool((grad_rows[-3:] == 0.25).all()) and bool((grad_rows[:, -1] == 0.25).all())
     want = rows[routing.places.view(-1).long(), 0].double().view(tokens, choices) * D
     assert_sum(grad_weights, want, want.abs(), D, F32)
@@ -255,7 +255,7 @@ def test_places_out_of_range_are_left_alone():
     offsets = torch.tensor([0, 50], dtype=torch.int32, device=DEV)  # claims more rows than there are
     rows = torch.arange(16, device=DEV, dtype=F32).view(4, 4)
     assert torch.equal(ops.expert_combine(rows, places, offsets), rows[:2])
-    grad_rows, grad_w = experts_mod._combine_backward(torch.ones(2, 4, device=DEV), rows, places, offsets,
+    grad_rows, grad_w = experts_mod.compiled().expert_combine_backward(torch.ones(2, 4, device=DEV), rows, places, offsets,
                                                       torch.ones(2, 2, device=DEV))
     assert torch.equal(grad_rows[:2], torch.ones(2, 4, device=DEV))
     assert grad_w.tolist() == [[6.0, 0.0], [0.0, 22.0]]
