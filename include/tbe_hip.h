@@ -640,8 +640,8 @@ TBE_API int tbe_backward_sgd_interleaved(const void *grad_output, void *weights,
  *   order           int32 [num_pairs]  pair at every place: those of expert 0 first, then expert 1, ..., then the
  *                                      dropped ones, ascending inside each
  *   places          int32 [num_pairs]  the inverse: place of every pair
- * The workspace (tbe_expert_plan_workspace_bytes; 0 for sizes that are refused) is free again after the call's
- * launches.
+ * The workspace (tbe_expert_plan_workspace_bytes; 0 for sizes that need none or are refused) is free again after
+ * the call's launches.
  *
  * Rows have D elements of `dtype` (TBE_DTYPE_F32, F16, F64 or BF16); the *_stride arguments are the elements
  * from one row of an input to the next (outputs are contiguous).  num_rows = num_tokens * choices.

@@ -86,11 +86,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> expert_plan(at::Tensor expert_ids
   at::Tensor places = at::empty(expert_ids.sizes(), ints);
   const uint64_t bytes = tbe_expert_plan_workspace_bytes(pairs, static_cast<int32_t>(num_experts));
   // (a call of its own scratch: two graphs captured on one stream do not share it)
-  at::Tensor scratch = at::empty({static_cast<int64_t>(bytes)}, expert_ids.options().dtype(at::kByte));
+  at::Tensor scratch;
+  if (bytes > 0) scratch = at::empty({static_cast<int64_t>(bytes)}, expert_ids.options().dtype(at::kByte));
   check(tbe_expert_plan(expert_ids.data_ptr(), static_cast<int32_t>(expert_ids.element_size()), pairs,
                         static_cast<int32_t>(num_experts), expert_offsets.data_ptr<int32_t>(),
-                        order.data_ptr<int32_t>(), places.data_ptr<int32_t>(), scratch.data_ptr(), bytes,
-                        stream_of(expert_ids)));
+                        order.data_ptr<int32_t>(), places.data_ptr<int32_t>(), bytes > 0 ? scratch.data_ptr() : nullptr,
+                        bytes, stream_of(expert_ids)));
   return {expert_offsets, order, places};
 }
 

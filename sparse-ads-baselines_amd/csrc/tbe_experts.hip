@@ -18,36 +18,50 @@ namespace tbe {
 namespace {
 
 // ------------------------------------------------------------------------------------ plan
-// A stable counting sort by expert.  Up to kSmallPairs pairs: one workgroup, one launch.  More: the
-// counts of every tile of pairs, their prefix sums over the tiles of an expert, and a launch that
-// ranks a tile's pairs with wavefront ballots (all lanes of one expert are found with one ballot per bit
-// of the expert's number) and places them.  Pairs inside a tile are numbered (wavefront, item, lane),
-// which the ranking keeps, so the order is stable.
+// A stable counting sort by expert.  What bounds it is latency: the whole input is a few MB at most, so launches,
+// barriers and chains of dependent steps are kept few.
+//   up to kFewPairs pairs   one workgroup, one launch
+//   few tiles               two launches: the counts of every tile of pairs; then every tile adds up the counts of
+//                           the tiles before it (and of all) itself.  Tiles of one pair a thread while that
+//                           reads few counts, of four beyond
+//   more                    three: a launch in between turns an expert's counts into prefix sums over the tiles
+// (Measured, 8 / 64 / 256 experts: 8192 pairs in one workgroup of eight pairs a thread 9.1 / 10.9 / 12.9 us, in two
+// launches with four pairs a thread 9.1 / 9.7 / 10.6, with one 6.3 / 6.7 / 7.6; 262144 pairs 7.3 / 9.0 / 14.2 with one, 9.9 /
+// 11.7 / 14.1 with four; 524288: 13.1 / 15.1 / 18.0, 10.5 / 12.1 / 15.6, and three launches 12.1 / 13.9 / 15.7.)
+// A tile's pairs are ranked with wavefront ballots (all lanes of one expert are found with one ballot per bit of the
+// expert's number).  Pairs inside a tile are numbered (wavefront, item, lane), which the ranking keeps, so the
+// order is stable.
 constexpr int kMaxExperts = TBE_MAX_EXPERTS;  // and one bin more for the dropped pairs
-constexpr int kTileWaves = 4, kTileItems = 8;
-constexpr int kPlanTile = kTileWaves * kWave * kTileItems;
-constexpr int kSmallWaves = 16, kSmallItems = 8;
-constexpr int kSmallPairs = kSmallWaves * kWave * kSmallItems;
-constexpr int kSmallExperts = 1023;  // widest single-workgroup plan: 16 wavefronts' counters in 64 KB of LDS
+constexpr int kTinyPairs = kWave;       // one wavefront
+constexpr int kFewPairs = 16 * kWave;
+constexpr int kFewExperts = 1023;       // widest plan with 16 wavefronts a workgroup: their counters take 64 KB of LDS
+constexpr int kManyItems = 4;           // pairs a thread of the larger tiles
+// wavefronts of a workgroup that ranks with `bins` counters per wavefront
+constexpr int tile_waves(int bins) { return bins <= 1024 ? 16 : 4; }
+constexpr int tile_pairs(int bins, int items) { return tile_waves(bins) * kWave * items; }
 
 template <typename I> __device__ __forceinline__ int bin_of(I expert, int E) {
   return (expert >= 0 && expert < E) ? static_cast<int>(expert) : E;
 }
 
-template <typename I, int BINS>
-__global__ __launch_bounds__(kBlockThreads) void expert_count_kernel(const I *__restrict__ ids, int64_t n, int E,
-                                                                    int64_t tiles, int32_t *__restrict__ counts) {
+// counts[tile][bin] (DIRECT) or counts[bin][tile]
+template <typename I, int ITEMS, int BINS, bool DIRECT>
+__global__ __launch_bounds__(tile_waves(BINS) * kWave) void expert_count_kernel(
+    const I *__restrict__ ids, int64_t n, int E, int64_t tiles, int32_t *__restrict__ counts) {
+  constexpr int kThreads = tile_waves(BINS) * kWave;
   __shared__ int32_t s_count[BINS];
-  for (int e = threadIdx.x; e <= E; e += kBlockThreads) s_count[e] = 0;
-  __syncthreads();
-  const int64_t base = static_cast<int64_t>(blockIdx.x) * kPlanTile + threadIdx.x;
+  const int64_t base = static_cast<int64_t>(blockIdx.x) * tile_pairs(BINS, ITEMS) + threadIdx.x;
+  I id[ITEMS];
 #pragma unroll
-  for (int q = 0; q < kTileItems; ++q) {
-    const int64_t a = base + q * kBlockThreads;
-    if (a < n) atomicAdd(&s_count[bin_of(ids[a], E)], 1);
-  }
+  for (int q = 0; q < ITEMS; ++q) id[q] = ids[min(base + q * kThreads, n - 1)];
+  for (int e = threadIdx.x; e <= E; e += kThreads) s_count[e] = 0;
   __syncthreads();
-  for (int e = threadIdx.x; e <= E; e += kBlockThreads) counts[e * tiles + blockIdx.x] = s_count[e];
+#pragma unroll
+  for (int q = 0; q < ITEMS; ++q)
+    if (base + q * kThreads < n) atomicAdd(&s_count[bin_of(id[q], E)], 1);
+  __syncthreads();
+  for (int e = threadIdx.x; e <= E; e += kThreads)
+    counts[DIRECT ? blockIdx.x * static_cast<int64_t>(E + 1) + e : e * tiles + blockIdx.x] = s_count[e];
 }
 
 // One wavefront per bin: exclusive prefix sums of its counts over the tiles, and its total.
@@ -72,7 +86,9 @@ __global__ __launch_bounds__(kBlockThreads) void expert_scan_kernel(int32_t *__r
   if (lane == 0) totals[e] = running;
 }
 
-template <typename I, int WAVES, int ITEMS, int BINS, bool SINGLE>
+enum { kPlanSingle, kPlanDirect, kPlanScanned };
+
+template <typename I, int WAVES, int ITEMS, int BINS, int MODE>
 __global__ __launch_bounds__(WAVES *kWave) void expert_place_kernel(
     const I *__restrict__ ids, int64_t n, int E, int bits, const int32_t *__restrict__ counts,
     const int32_t *__restrict__ totals, int64_t tiles, int32_t *__restrict__ expert_offsets,
@@ -80,11 +96,10 @@ __global__ __launch_bounds__(WAVES *kWave) void expert_place_kernel(
   constexpr int kThreads = WAVES * kWave;
   __shared__ int32_t s_count[WAVES][BINS];
   __shared__ int32_t s_start[BINS];
+  __shared__ int32_t s_before[MODE == kPlanDirect ? BINS : 1];
   __shared__ int32_t s_wave[WAVES];
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = threadIdx.x >> 6;
-  for (int e = lane; e <= E; e += kWave) s_count[wave][e] = 0;
-  __syncthreads();
 
   const int64_t base = (static_cast<int64_t>(blockIdx.x) * WAVES + wave) * (kWave * ITEMS) + lane;
   int key[ITEMS], rank[ITEMS];
@@ -93,15 +108,40 @@ __global__ __launch_bounds__(WAVES *kWave) void expert_place_kernel(
     const int64_t a = base + q * kWave;
     key[q] = a < n ? bin_of(ids[a], E) : -1;
   }
+  for (int e = lane; e <= E; e += kWave) s_count[wave][e] = 0;
+  if constexpr (MODE == kPlanDirect) {
+    for (int e = threadIdx.x; e < BINS; e += kThreads) s_start[e] = s_before[e] = 0;
+  }
+  __syncthreads();
+  if constexpr (MODE == kPlanDirect) {
+    // threads are dealt to (bin, every parts-th tile); sums of whole numbers, whose order does not matter
+    const int wide = E + 1 < kThreads ? E + 1 : kThreads;
+    const int parts = kThreads / wide;
+    const int part = threadIdx.x / wide;
+    if (part < parts) {
+      for (int e = threadIdx.x - part * wide; e <= E; e += wide) {
+        int total = 0, before = 0;
+#pragma unroll 8
+        for (int t = part; t < static_cast<int>(tiles); t += parts) {
+          const int c = counts[t * (E + 1) + e];
+          total += c;
+          before += t < static_cast<int>(blockIdx.x) ? c : 0;
+        }
+        atomicAdd(&s_start[e], total);
+        atomicAdd(&s_before[e], before);
+      }
+    }
+  }
 #pragma unroll
   for (int q = 0; q < ITEMS; ++q) {
+    rank[q] = 0;
+    if (base - lane + q * kWave >= n) continue;  // (the whole wavefront)
     uint64_t same = __ballot(key[q] >= 0);
     for (int b = 0; b < bits; ++b) {
       const bool set = (key[q] >> b) & 1;
       const uint64_t vote = __ballot(set);
       same &= set ? vote : ~vote;
     }
-    rank[q] = 0;
     if (key[q] >= 0) {
       const int first = __ffsll(static_cast<unsigned long long>(same)) - 1;
       int before = 0;
@@ -121,9 +161,9 @@ __global__ __launch_bounds__(WAVES *kWave) void expert_place_kernel(
         s_count[w][e] = sum;
         sum += c;
       }
-      if constexpr (!SINGLE) sum = totals[e];
+      if constexpr (MODE == kPlanScanned) sum = totals[e];
     }
-    s_start[e] = sum;
+    if constexpr (MODE != kPlanDirect) s_start[e] = sum;
   }
   __syncthreads();
   // exclusive prefix sum over the bins
@@ -152,7 +192,8 @@ __global__ __launch_bounds__(WAVES *kWave) void expert_place_kernel(
     if (e <= E) {
       if (blockIdx.x == 0) expert_offsets[e] = start;
       int first = start;
-      if constexpr (!SINGLE) first += counts[e * tiles + blockIdx.x];
+      if constexpr (MODE == kPlanDirect) first += s_before[e];
+      if constexpr (MODE == kPlanScanned) first += counts[e * tiles + blockIdx.x];
       s_start[e] = first;
     }
     start += mine[i];
@@ -170,171 +211,220 @@ __global__ __launch_bounds__(WAVES *kWave) void expert_place_kernel(
 }
 
 // ------------------------------------------------------------------------------- row traffic
-// Rows are moved as vectors of VEC elements, the widest of 16, 8, 4 and 2 bytes that divides the row and
-// every address.  A workgroup takes `group` whole tokens, or, for rows of more than a workgroup's
-// vectors, one slice of one token (blockIdx.y); its threads are dealt to the (token, vector) pairs in
-// order, so that no lane idles for a row that is no power of two.
-struct RowTiles {
+// What bounds these kernels is memory: they move rows and do next to nothing with them.
+//
+// Rows are moved 16 bytes a lane, whatever their width and alignment: the memory system takes 16-byte accesses at
+// any element's address, and the last vector of a row is the one that ENDS with the row (it overlaps the one
+// before it; both write the same bytes).  Measured, 32768 tokens, 8 rows each, bf16, 2046 elements a row:
+// combined in 189 us that way, in 372 us with the 4-byte vectors that would divide the row.  Rows of fewer than
+// 16 bytes are moved element by element.
+//
+// One thread per (token, vector), numbered token after token, so that no lane idles for a row that is no power
+// of two wide; a thread asks for the places of up to eight choices, then for their eight rows, before it
+// uses the first.
+//
+// Row sets that the 256 MB memory-side cache cannot hold anyway are moved with streaming accesses (read, and, where a
+// row fills whole cache lines, written): 1.07 GB of rows of 4 KB dispatched in 205 us instead of 227, combined
+// in 184 instead of 218; but 67 MB dispatched and combined again 30.2 us without, 28.7 to 32.4 with them, and rows
+// of 4092 bytes 299 us streamed instead of 271 (partly written lines).
+struct RowMap {
   int64_t tokens;
-  int64_t groups;    // of `group` tokens; a workgroup takes every gridDim.x-th one
+  int64_t first;      // of this launch
   int32_t choices;
-  int32_t vectors;   // of a row
-  int32_t group;     // tokens of a workgroup
-  int32_t slice;     // vectors of a workgroup (group * vectors, or fewer than a row)
-  uint32_t magic;    // i / vectors = (i * magic) >> shift for the i < 2^16 that occur
+  int32_t vectors;    // of a row
+  int32_t D;          // elements of a row (bytes for dispatch)
+  uint32_t count;     // (token, vector) pairs of this launch, < 2^31
+  uint32_t magic;     // i / vectors = (i * magic) >> shift for i < 2^31
   int32_t shift;
 };
 
-__device__ __forceinline__ int divided(const RowTiles &r, int i) {
-  return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(i)) * r.magic) >> r.shift);
-}
+// 16 bytes at the address of any 2-byte element
+typedef uint32_t Words16 __attribute__((ext_vector_type(4), aligned(2)));
 
-template <typename T, int VEC> struct alignas(sizeof(T) * VEC) Pack {
+template <typename T, int VEC> struct Pack {
   T v[VEC];
 };
+template <typename T, int VEC, bool STREAM>
+__device__ __forceinline__ Pack<T, VEC> load_pack(const T *p) {
+  if constexpr (VEC == 1) {
+    return Pack<T, VEC>{{*p}};
+  } else {
+    static_assert(sizeof(Pack<T, VEC>) == 16, "full vectors");
+    const Words16 *w = reinterpret_cast<const Words16 *>(p);
+    Words16 x;
+    if constexpr (STREAM) x = __builtin_nontemporal_load(w);
+    else x = *w;
+    return __builtin_bit_cast(Pack<T, VEC>, x);
+  }
+}
+template <typename T, int VEC, bool STREAM>
+__device__ __forceinline__ void store_pack(T *p, const Pack<T, VEC> &v) {
+  if constexpr (VEC == 1) {
+    *p = v.v[0];
+  } else {
+    Words16 *w = reinterpret_cast<Words16 *>(p);
+    if constexpr (STREAM) __builtin_nontemporal_store(__builtin_bit_cast(Words16, v), w);
+    else *w = __builtin_bit_cast(Words16, v);
+  }
+}
 
-// The row of a pair, or -1 for one that is dropped.
+// A dropped pair's place lies behind the rows kept; so do places that are none.
 __device__ __forceinline__ bool is_kept(int32_t place, int32_t kept) {
   return static_cast<uint32_t>(place) < static_cast<uint32_t>(kept);
 }
+__device__ __forceinline__ int32_t rows_kept(const int32_t *kept_rows, int64_t pairs) {
+  return static_cast<int32_t>(min(static_cast<int64_t>(*kept_rows), pairs));
+}
 
-template <typename U, int ITER>
+// U: what is moved per lane (Words16, or one element of 2, 4 or 8 bytes)
+template <typename U, bool STREAM>
 __global__ __launch_bounds__(kBlockThreads) void expert_dispatch_kernel(
-    const U *__restrict__ x, int64_t x_stride, const int32_t *__restrict__ places,
-    const int32_t *__restrict__ kept_rows, U *__restrict__ rows, RowTiles r) {
-  const int col0 = blockIdx.y * r.slice;
-  const int64_t pairs = r.tokens * r.choices;
+    const char *__restrict__ x, int64_t x_stride, const int32_t *__restrict__ places,
+    const int32_t *__restrict__ kept_rows, char *__restrict__ rows, RowMap m) {
+  constexpr int kAhead = 8;
+  const uint32_t i = blockIdx.x * kBlockThreads + threadIdx.x;
+  if (i >= m.count) return;
+  const uint32_t t = static_cast<uint32_t>((static_cast<uint64_t>(i) * m.magic) >> m.shift);
+  const int col = min(static_cast<int>((i - t * m.vectors) * sizeof(U)), m.D - static_cast<int>(sizeof(U)));
+  const int64_t token = m.first + t;
+  const uint32_t pairs = static_cast<uint32_t>(m.tokens * m.choices);
   const int32_t kept = *kept_rows;
-  for (int64_t group = blockIdx.x; group < r.groups; group += gridDim.x) {
+  const U v = *reinterpret_cast<const U *>(x + token * x_stride + col);
+  const int32_t *mine = places + token * m.choices;
+  for (int j0 = 0; j0 < m.choices; j0 += kAhead) {
+    int32_t place[kAhead];
 #pragma unroll
-    for (int it = 0; it < ITER; ++it) {
-      const int i = it * kBlockThreads + threadIdx.x;
-      if (i >= r.slice) continue;
-      const int t = r.group > 1 ? divided(r, i) : 0;
-      const int col = col0 + i - t * r.vectors;
-      const int64_t token = group * r.group + t;
-      if (token >= r.tokens || col >= r.vectors) continue;
-      const U v = x[token * x_stride + col];
-      for (int j = 0; j < r.choices; ++j) {
-        const int32_t place = places[token * r.choices + j];
-        if (place < 0 || place >= pairs) continue;
-        rows[static_cast<int64_t>(place) * r.vectors + col] = place < kept ? v : U{};
-      }
+    for (int j = 0; j < kAhead; ++j) place[j] = j0 + j < m.choices ? mine[j0 + j] : -1;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (static_cast<uint32_t>(place[j]) >= pairs) continue;
+      U *to = reinterpret_cast<U *>(rows + static_cast<int64_t>(place[j]) * m.D + col);
+      const U o = place[j] < kept ? v : U{};
+      if constexpr (STREAM) __builtin_nontemporal_store(o, to);
+      else *to = o;
     }
   }
 }
 
-template <typename T, typename W, int VEC, int ITER>
+template <typename T, typename W, int VEC, int AHEAD, bool STREAM>
 __global__ __launch_bounds__(kBlockThreads) void expert_combine_kernel(
     const T *__restrict__ rows, int64_t row_stride, const int32_t *__restrict__ places,
-    const int32_t *__restrict__ kept_rows, const W *__restrict__ weights, T *__restrict__ out, RowTiles r) {
+    const int32_t *__restrict__ kept_rows, const W *__restrict__ weights, T *__restrict__ out, RowMap m) {
   using A = typename AccOf<T>::type;
   using P = Pack<T, VEC>;
-  const int col0 = blockIdx.y * r.slice;
-  const int32_t kept = static_cast<int32_t>(min(static_cast<int64_t>(*kept_rows), r.tokens * r.choices));
-  for (int64_t group = blockIdx.x; group < r.groups; group += gridDim.x) {
+  const uint32_t i = blockIdx.x * kBlockThreads + threadIdx.x;
+  if (i >= m.count) return;
+  const uint32_t t = static_cast<uint32_t>((static_cast<uint64_t>(i) * m.magic) >> m.shift);
+  const int col = min(static_cast<int>(i - t * m.vectors) * VEC, m.D - VEC);
+  const int64_t token = m.first + t;
+  const int32_t kept = rows_kept(kept_rows, m.tokens * m.choices);
+  A sum[VEC];
 #pragma unroll
-    for (int it = 0; it < ITER; ++it) {
-      const int i = it * kBlockThreads + threadIdx.x;
-      if (i >= r.slice) continue;
-      const int t = r.group > 1 ? divided(r, i) : 0;
-      const int col = col0 + i - t * r.vectors;
-      const int64_t token = group * r.group + t;
-      if (token >= r.tokens || col >= r.vectors) continue;
-      A sum[VEC];
+  for (int q = 0; q < VEC; ++q) sum[q] = A(0);
+  for (int j0 = 0; j0 < m.choices; j0 += AHEAD) {
+    int32_t place[AHEAD];
+    A w[AHEAD];
 #pragma unroll
-      for (int q = 0; q < VEC; ++q) sum[q] = A(0);
-      for (int j = 0; j < r.choices; ++j) {
-        const int64_t a = token * r.choices + j;
-        const int32_t place = places[a];
-        if (!is_kept(place, kept)) continue;
-        const P v = *reinterpret_cast<const P *>(rows + place * row_stride + static_cast<int64_t>(col) * VEC);
-        const A w = weights ? static_cast<A>(weights[a]) : A(1);
+    for (int j = 0; j < AHEAD; ++j) {
+      const int64_t a = token * m.choices + min(j0 + j, m.choices - 1);  // clamped: no branch per load
+      place[j] = places[a];
+      w[j] = weights ? static_cast<A>(weights[a]) : A(1);
+    }
+    P v[AHEAD];
+    bool keep[AHEAD];
 #pragma unroll
-        for (int q = 0; q < VEC; ++q) sum[q] += w * static_cast<A>(v.v[q]);
-      }
-      P o;
+    for (int j = 0; j < AHEAD; ++j) {
+      keep[j] = j0 + j < m.choices && is_kept(place[j], kept);
+      // (a dropped pair asks for row 0, which stays in the caches, and drops it: no branch between the loads)
+      v[j] = load_pack<T, VEC, STREAM>(rows + (keep[j] ? place[j] : 0) * row_stride + col);
+    }
 #pragma unroll
-      for (int q = 0; q < VEC; ++q) o.v[q] = static_cast<T>(sum[q]);
-      *reinterpret_cast<P *>(out + (token * r.vectors + col) * VEC) = o;
+    for (int j = 0; j < AHEAD; ++j) {
+#pragma unroll
+      for (int q = 0; q < VEC; ++q) sum[q] = keep[j] ? sum[q] + w[j] * static_cast<A>(v[j].v[q]) : sum[q];
     }
   }
+  P o;
+#pragma unroll
+  for (int q = 0; q < VEC; ++q) o.v[q] = static_cast<T>(sum[q]);
+  store_pack<T, VEC, false>(out + token * m.D + col, o);
 }
 
-// GROUP lanes per token (a workgroup per token for GROUP = 256): the token's gradient row is read once per
-// kChoices choices, every chosen row is read and its gradient written once.  Without grad_weights the rows are
-// not read, without grad_rows nothing is written to them.
-template <typename T, typename W, int VEC, int GROUP>
+// GROUP lanes per pair (a workgroup per pair for GROUP = 256): the pair's row is read once, its gradient written
+// once; the token's gradient row comes from the caches for all pairs of the token but the first.  (One group per
+// token, its gradient row held in registers over four choices at a time, took 485 us where this takes 447: 32768
+// tokens, 8 rows of 2048 bf16 each.)  Without grad_weights the rows are not read, without grad_rows nothing is
+// written to them.
+template <typename T, typename W, int VEC, int GROUP, bool STREAM>
 __global__ __launch_bounds__(kBlockThreads) void expert_combine_backward_kernel(
     const T *__restrict__ grad, int64_t grad_stride, const T *__restrict__ rows, int64_t row_stride,
     const int32_t *__restrict__ places, const int32_t *__restrict__ kept_rows, const W *__restrict__ weights,
-    T *__restrict__ grad_rows, W *__restrict__ grad_weights, int64_t tokens, int choices, int vectors) {
+    T *__restrict__ grad_rows, W *__restrict__ grad_weights, uint32_t pairs, int64_t slots, int choices, int vectors,
+    int D, uint32_t magic, int shift) {
   using A = typename AccOf<T>::type;
   using P = Pack<T, VEC>;
-  constexpr int kChoices = 4;
-  __shared__ A s_part[kWavesPerBlock][kChoices];
+  constexpr int kPairs = kBlockThreads / GROUP;
+  __shared__ A s_part[kWavesPerBlock];
   const int sub = threadIdx.x % GROUP;
-  constexpr int kTokens = kBlockThreads / GROUP;
-  const int64_t pairs = tokens * choices;
-  const int32_t kept = static_cast<int32_t>(min(static_cast<int64_t>(*kept_rows), pairs));
+  const int32_t kept = rows_kept(kept_rows, pairs);
   // (a group leaves as a whole; with GROUP = 256 the workgroup does, so that its barriers are met by all or none)
-  for (int64_t token = static_cast<int64_t>(blockIdx.x) * kTokens + threadIdx.x / GROUP; token < tokens;
-       token += static_cast<int64_t>(gridDim.x) * kTokens)
-  for (int j0 = 0; j0 < choices; j0 += kChoices) {
-    const T *g_row = grad + token * grad_stride;
-    int32_t place[kChoices];
-    A w[kChoices], dot[kChoices];
-#pragma unroll
-    for (int j = 0; j < kChoices; ++j) {
-      const int64_t a = token * choices + j0 + j;
-      place[j] = j0 + j < choices ? places[a] : -1;
-      if (place[j] >= pairs) place[j] = -1;
-      w[j] = is_kept(place[j], kept) ? static_cast<A>(weights[a]) : A(0);
-      dot[j] = A(0);
+  for (int64_t at = static_cast<int64_t>(blockIdx.x) * kPairs + threadIdx.x / GROUP; at < slots;
+       at += static_cast<int64_t>(gridDim.x) * kPairs) {
+    int64_t pair = at;
+    uint32_t token;
+    if constexpr (GROUP > kWave) {
+      // workgroups are dealt to the XCDs in turn: a token's pairs go to every eighth one, so that its gradient row is
+      // fetched into one L2 and not into as many as the token has choices
+      const uint32_t q = static_cast<uint32_t>((static_cast<uint64_t>(at >> 3) * magic) >> shift);  // of 8 * choices
+      const uint32_t j = static_cast<uint32_t>(at >> 3) - q * choices;
+      token = q * kNumXcd + static_cast<uint32_t>(at & (kNumXcd - 1));
+      pair = static_cast<int64_t>(token) * choices + j;
+      if (pair >= pairs) continue;
+    } else {
+      token = static_cast<uint32_t>((static_cast<uint64_t>(pair) * magic) >> shift);
     }
-    for (int col = sub; col < vectors; col += GROUP) {
-      const P gv = *reinterpret_cast<const P *>(g_row + static_cast<int64_t>(col) * VEC);
-#pragma unroll
-      for (int j = 0; j < kChoices; ++j) {
-        if (place[j] < 0) continue;
-        const bool keep = place[j] < kept;
+    const int32_t place = places[pair];
+    const bool keep = is_kept(place, kept);
+    const bool write = grad_rows && static_cast<uint32_t>(place) < pairs;
+    const A w = keep ? static_cast<A>(weights[pair]) : A(0);
+    const T *g_row = grad + token * grad_stride;
+    const T *row = rows + place * row_stride;
+    T *to = grad_rows + static_cast<int64_t>(place) * D;
+    A dot = A(0);
+    for (int c = sub; c < vectors; c += GROUP) {
+      const int col = min(c * VEC, D - VEC);
+      const int seen = c * VEC - col;  // elements that the row's last vector shares with the one before it
+      P g, v;
+      if (keep) {
+        g = load_pack<T, VEC, false>(g_row + col);
+        if (grad_weights) v = load_pack<T, VEC, STREAM>(row + col);
+      }
+      if (write) {
         P o;
-        if (keep && grad_weights) {
-          const P v = *reinterpret_cast<const P *>(rows + place[j] * row_stride + static_cast<int64_t>(col) * VEC);
 #pragma unroll
-          for (int q = 0; q < VEC; ++q) dot[j] += static_cast<A>(v.v[q]) * static_cast<A>(gv.v[q]);
+        for (int q = 0; q < VEC; ++q) o.v[q] = keep ? static_cast<T>(w * static_cast<A>(g.v[q])) : T(0);
+        store_pack<T, VEC, false>(to + col, o);
+      }
+      if (grad_weights && keep) {
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) {
+          const A term = static_cast<A>(v.v[q]) * static_cast<A>(g.v[q]);
+          dot += q >= seen ? term : A(0);
         }
-        if (!grad_rows) continue;
-#pragma unroll
-        for (int q = 0; q < VEC; ++q) o.v[q] = keep ? static_cast<T>(w[j] * static_cast<A>(gv.v[q])) : T(0);
-        *reinterpret_cast<P *>(grad_rows + (static_cast<int64_t>(place[j]) * vectors + col) * VEC) = o;
       }
     }
     if (!grad_weights) continue;
 #pragma unroll
-    for (int j = 0; j < kChoices; ++j) {
-#pragma unroll
-      for (int m = 1; m < (GROUP < kWave ? GROUP : kWave); m <<= 1) dot[j] += shfl_x(dot[j], m);
-    }
+    for (int d = 1; d < (GROUP < kWave ? GROUP : kWave); d <<= 1) dot += shfl_x(dot, d);
     if constexpr (GROUP > kWave) {
       __syncthreads();
-      if ((threadIdx.x & (kWave - 1)) == 0) {
-#pragma unroll
-        for (int j = 0; j < kChoices; ++j) s_part[threadIdx.x >> 6][j] = dot[j];
-      }
+      if ((threadIdx.x & (kWave - 1)) == 0) s_part[threadIdx.x >> 6] = dot;
       __syncthreads();
+      dot = A(0);
 #pragma unroll
-      for (int j = 0; j < kChoices; ++j) {
-        dot[j] = A(0);
-#pragma unroll
-        for (int q = 0; q < kWavesPerBlock; ++q) dot[j] += s_part[q][j];
-      }
+      for (int q = 0; q < kWavesPerBlock; ++q) dot += s_part[q];
     }
-    if (sub == 0) {
-#pragma unroll
-      for (int j = 0; j < kChoices; ++j)
-        if (j0 + j < choices) grad_weights[token * choices + j0 + j] = static_cast<W>(dot[j]);
-    }
+    if (sub == 0) grad_weights[pair] = static_cast<W>(dot);
   }
 }
 
@@ -346,43 +436,38 @@ bool float_dtype(int32_t dtype) {
   return dtype == TBE_DTYPE_F32 || dtype == TBE_DTYPE_F16 || dtype == TBE_DTYPE_F64 || dtype == TBE_DTYPE_BF16;
 }
 
-// Widest power of two up to 16 that divides all of the byte counts and addresses or'ed into `bits`.
-int vector_bytes(uint64_t bits) {
-  int v = 16;
-  while (bits & (v - 1)) v >>= 1;
-  return v;
-}
 uint64_t address(const void *p) { return reinterpret_cast<uint64_t>(p); }
 
-constexpr int kRowIter = 4;  // vectors per thread
-constexpr int64_t kMaxGrid = 1 << 22;  // workgroups of a launch: grid times workgroup stays below 2^32 threads
+// Rows that the memory-side cache (256 MB) does not hold are streamed.
+bool streams(int64_t pairs, int64_t row_bytes) { return pairs * row_bytes > (int64_t{256} << 20); }
+// Streamed stores: only where they fill whole cache lines.
+bool whole_lines(const void *base, int64_t row_bytes) { return ((address(base) | row_bytes) & 127) == 0; }
 
-// (the division is exact: i < 2^16 and vectors <= 2^16 where it is used)
-RowTiles row_tiles(int64_t tokens, int32_t choices, int64_t vectors, dim3 *grid) {
-  RowTiles r;
-  r.tokens = tokens;
-  r.choices = choices;
-  r.vectors = static_cast<int32_t>(vectors);
-  constexpr int64_t kSpan = kBlockThreads * kRowIter;
-  if (vectors >= kSpan) {
-    r.group = 1;
-    r.groups = tokens;
-    r.slice = static_cast<int32_t>(kSpan);
-    r.magic = 0;
-    r.shift = 0;
-    *grid = dim3(static_cast<unsigned>(std::min(tokens, kMaxGrid)), static_cast<unsigned>(ceil_div(vectors, kSpan)));
-    return r;
-  }
-  r.group = static_cast<int32_t>(kSpan / vectors);
-  r.slice = static_cast<int32_t>(r.group * vectors);
+// i / d = (i * magic) >> shift for i < 2^31: magic = ceil(2^(31 + s) / d) with s = ceil(log2 d) fits 32 bits, and its
+// error of less than d / 2^(31 + s) <= 2^-31 a unit of i stays below 1 / d for every such i.
+void division_by(int64_t d, uint32_t *magic, int32_t *shift) {
   int log2 = 0;
-  while ((int64_t{1} << log2) < vectors) ++log2;
-  r.shift = 16 + log2;
-  r.magic = static_cast<uint32_t>(((uint64_t{1} << r.shift) + vectors - 1) / vectors);
-  r.groups = ceil_div(tokens, r.group);
-  *grid = dim3(static_cast<unsigned>(std::min(r.groups, kMaxGrid)));
-  return r;
+  while ((int64_t{1} << log2) < d) ++log2;
+  *shift = 31 + log2;
+  *magic = static_cast<uint32_t>(((uint64_t{1} << *shift) + static_cast<uint64_t>(d) - 1) / static_cast<uint64_t>(d));
 }
+
+// f(map, grid) for every launch of at most 2^31 - 1 threads, each over whole tokens.
+template <typename F> void for_row_maps(int64_t tokens, int32_t choices, int64_t vectors, int64_t D, F &&f) {
+  RowMap m;
+  m.tokens = tokens;
+  m.choices = choices;
+  m.vectors = static_cast<int32_t>(vectors);
+  m.D = static_cast<int32_t>(D);
+  division_by(vectors, &m.magic, &m.shift);
+  const int64_t most = std::max<int64_t>(1, (INT32_MAX - kBlockThreads) / vectors);
+  for (m.first = 0; m.first < tokens; m.first += most) {
+    m.count = static_cast<uint32_t>(std::min(most, tokens - m.first) * vectors);
+    f(m, dim3(static_cast<unsigned>(ceil_div(m.count, kBlockThreads))));
+  }
+}
+
+constexpr int64_t kMaxGrid = 1 << 22;  // workgroups of a launch: grid times workgroup stays below 2^32 threads
 
 int plan_bits(int32_t experts) {  // bits of the largest bin number, `experts`
   int bits = 0;
@@ -390,35 +475,60 @@ int plan_bits(int32_t experts) {  // bits of the largest bin number, `experts`
   return bits;
 }
 
+// Bins of the kernels that serve `experts`, which has to stay below them.
+int plan_bins(int32_t experts) { return experts < 256 ? 256 : experts < 1024 ? 1024 : 4096; }
+
 struct PlanRegions {
-  uint64_t counts, totals, total_bytes;
-  int64_t tiles;
+  uint64_t totals, total_bytes;  // (the counts come first)
+  int64_t tiles;                 // 0: one workgroup
+  int items;                     // pairs a thread
+  bool direct;                   // no launch for the prefix sums
 };
 PlanRegions plan_regions(int64_t pairs, int32_t experts) {
-  PlanRegions p;
-  p.tiles = 0;
-  p.counts = p.totals = 0;
-  p.total_bytes = 256;
-  if (pairs <= kSmallPairs && experts <= kSmallExperts) return p;
-  p.tiles = std::max<int64_t>(1, ceil_div(pairs, kPlanTile));
+  PlanRegions p{0, 0, 0, 1, true};
+  if (pairs <= kFewPairs && experts <= kFewExperts) return p;
+  const int bins = plan_bins(experts);
+  // tiles whose counts each of them may add up itself
+  const auto few = [&](int64_t most) { return std::min<int64_t>(most, (1 << 16) / (experts + 1)); };
+  p.tiles = std::max<int64_t>(1, ceil_div(pairs, tile_pairs(bins, 1)));
+  if (p.tiles > few(256)) {
+    p.items = kManyItems;
+    p.tiles = ceil_div(pairs, tile_pairs(bins, kManyItems));
+    p.direct = p.tiles <= few(128);
+  }
   p.totals = align_up(static_cast<uint64_t>(p.tiles) * (experts + 1) * 4, 256);
-  p.total_bytes = p.totals + align_up((experts + 1) * 4ull, 256);
+  // (at least what the smaller tiles take, so that a workspace sized for a maximum serves every smaller batch)
+  const uint64_t smaller = p.items > 1 ? align_up(static_cast<uint64_t>(few(256)) * (experts + 1) * 4, 256) : 0;
+  p.total_bytes = std::max(p.totals, smaller) + align_up((experts + 1) * 4ull, 256);
   return p;
 }
 
 template <typename I, int BINS>
 void launch_plan_tiles(const I *ids, int64_t pairs, int32_t experts, const PlanRegions &p, void *workspace,
                        int32_t *expert_offsets, int32_t *order, int32_t *places, hipStream_t s) {
-  int32_t *counts = reinterpret_cast<int32_t *>(static_cast<char *>(workspace) + p.counts);
+  int32_t *counts = static_cast<int32_t *>(workspace);
   int32_t *totals = reinterpret_cast<int32_t *>(static_cast<char *>(workspace) + p.totals);
-  const dim3 grid(static_cast<unsigned>(p.tiles));
-  TBE_LAUNCH("expert_count", s, (expert_count_kernel<I, BINS>), grid, dim3(kBlockThreads), ids, pairs, experts,
-             p.tiles, counts);
-  TBE_LAUNCH("expert_scan", s, expert_scan_kernel, dim3(static_cast<unsigned>(ceil_div(experts + 1, kWavesPerBlock))),
-             dim3(kBlockThreads), counts, p.tiles, experts, totals);
-  TBE_LAUNCH("expert_place", s, (expert_place_kernel<I, kTileWaves, kTileItems, BINS, false>), grid,
-             dim3(kTileWaves * kWave), ids, pairs, experts, plan_bits(experts), counts, totals, p.tiles,
-             expert_offsets, order, places);
+  const dim3 grid(static_cast<unsigned>(p.tiles)), block(tile_waves(BINS) * kWave);
+#define TBE_PLAN_COUNT(ITEMS, DIRECT)                                                                             \
+  TBE_LAUNCH("expert_count", s, (expert_count_kernel<I, ITEMS, BINS, DIRECT>), grid, block, ids, pairs, experts, \
+             p.tiles, counts)
+#define TBE_PLAN_PLACE(ITEMS, MODE)                                                                               \
+  TBE_LAUNCH("expert_place", s, (expert_place_kernel<I, tile_waves(BINS), ITEMS, BINS, MODE>), grid, block, ids,  \
+             pairs, experts, plan_bits(experts), counts, totals, p.tiles, expert_offsets, order, places)
+  if (p.items == 1) {
+    TBE_PLAN_COUNT(1, true);
+    TBE_PLAN_PLACE(1, kPlanDirect);
+  } else if (p.direct) {
+    TBE_PLAN_COUNT(kManyItems, true);
+    TBE_PLAN_PLACE(kManyItems, kPlanDirect);
+  } else {
+    TBE_PLAN_COUNT(kManyItems, false);
+    TBE_LAUNCH("expert_scan", s, expert_scan_kernel, dim3(static_cast<unsigned>(ceil_div(experts + 1, kWavesPerBlock))),
+               dim3(kBlockThreads), counts, p.tiles, experts, totals);
+    TBE_PLAN_PLACE(kManyItems, kPlanScanned);
+  }
+#undef TBE_PLAN_COUNT
+#undef TBE_PLAN_PLACE
 }
 
 template <typename I>
@@ -427,19 +537,20 @@ void launch_plan(const void *expert_ids, int64_t pairs, int32_t experts, const P
   const I *ids = static_cast<const I *>(expert_ids);
   if (p.tiles == 0) {
     const int32_t *none = nullptr;
-#define TBE_PLAN_SMALL(BINS)                                                                                     \
-  TBE_LAUNCH("expert_place", s, (expert_place_kernel<I, kSmallWaves, kSmallItems, BINS, true>), dim3(1),         \
-             dim3(kSmallWaves * kWave), ids, pairs, experts, plan_bits(experts), none, none, int64_t{1},         \
+#define TBE_PLAN_FEW(WAVES, BINS)                                                                                \
+  TBE_LAUNCH("expert_place", s, (expert_place_kernel<I, WAVES, 1, BINS, kPlanSingle>), dim3(1),                  \
+             dim3(WAVES *kWave), ids, pairs, experts, plan_bits(experts), none, none, int64_t{1},                \
              expert_offsets, order, places)
-    if (experts < 256) { TBE_PLAN_SMALL(256); }
-    else { TBE_PLAN_SMALL(1024); }
-#undef TBE_PLAN_SMALL
-  } else if (experts < 256) {
-    launch_plan_tiles<I, 256>(ids, pairs, experts, p, workspace, expert_offsets, order, places, s);
-  } else if (experts < 1024) {
-    launch_plan_tiles<I, 1024>(ids, pairs, experts, p, workspace, expert_offsets, order, places, s);
-  } else {
-    launch_plan_tiles<I, 4096>(ids, pairs, experts, p, workspace, expert_offsets, order, places, s);
+    if (experts < 256 && pairs <= kTinyPairs) { TBE_PLAN_FEW(1, 256); }
+    else if (experts < 256) { TBE_PLAN_FEW(16, 256); }
+    else { TBE_PLAN_FEW(16, 1024); }
+#undef TBE_PLAN_FEW
+    return;
+  }
+  switch (plan_bins(experts)) {
+    case 256: return launch_plan_tiles<I, 256>(ids, pairs, experts, p, workspace, expert_offsets, order, places, s);
+    case 1024: return launch_plan_tiles<I, 1024>(ids, pairs, experts, p, workspace, expert_offsets, order, places, s);
+    default: return launch_plan_tiles<I, 4096>(ids, pairs, experts, p, workspace, expert_offsets, order, places, s);
   }
 }
 
@@ -455,52 +566,89 @@ struct CombineCall {
   hipStream_t stream;
 };
 
-template <typename T, typename W, int VEC>
-void launch_combine(const CombineCall &c, void *output) {
-  dim3 grid;
-  const RowTiles r = row_tiles(c.tokens, c.choices, c.D / VEC, &grid);
-  TBE_LAUNCH("expert_combine", c.stream, (expert_combine_kernel<T, W, VEC, kRowIter>), grid, dim3(kBlockThreads),
-             static_cast<const T *>(c.rows), c.row_stride, c.places, c.kept, static_cast<const W *>(c.weights),
-             static_cast<T *>(output), r);
+template <typename T, typename W, int VEC, int AHEAD, bool STREAM>
+void launch_combine_as(const CombineCall &c, void *output) {
+  for_row_maps(c.tokens, c.choices, ceil_div(c.D, VEC), c.D, [&](const RowMap &m, dim3 grid) {
+    TBE_LAUNCH("expert_combine", c.stream, (expert_combine_kernel<T, W, VEC, AHEAD, STREAM>), grid, dim3(kBlockThreads),
+               static_cast<const T *>(c.rows), c.row_stride, c.places, c.kept, static_cast<const W *>(c.weights),
+               static_cast<T *>(output), m);
+  });
+}
+
+template <typename T, typename W, int VEC> void launch_combine(const CombineCall &c, void *output) {
+  if constexpr (VEC == 1) {
+    launch_combine_as<T, W, 1, 4, false>(c, output);
+  } else {
+    const bool stream = streams(c.tokens * c.choices, c.D * sizeof(T));
+#define TBE_COMBINE(AHEAD)                                                          \
+  do {                                                                              \
+    if (stream) launch_combine_as<T, W, VEC, AHEAD, true>(c, output);               \
+    else launch_combine_as<T, W, VEC, AHEAD, false>(c, output);                     \
+  } while (0)
+    if (c.choices <= 2) TBE_COMBINE(2);
+    else if (c.choices <= 4) TBE_COMBINE(4);
+    else TBE_COMBINE(8);
+#undef TBE_COMBINE
+  }
+}
+
+template <typename T, typename W, int VEC, bool STREAM>
+void launch_combine_backward_as(const CombineCall &c, const void *grad, int64_t grad_stride, void *grad_rows,
+                                void *grad_weights) {
+  const int vectors = static_cast<int>(ceil_div(c.D, VEC));
+  const int64_t pairs = c.tokens * c.choices;
+  uint32_t magic;
+  int shift;
+  division_by(c.choices, &magic, &shift);
+  int64_t slots = pairs;
+#define TBE_COMBINE_BACKWARD(GROUP)                                                                                \
+  TBE_LAUNCH("expert_combine_backward", c.stream, (expert_combine_backward_kernel<T, W, VEC, GROUP, STREAM>),      \
+             dim3(static_cast<unsigned>(std::min(ceil_div(slots, kBlockThreads / GROUP), kMaxGrid))),              \
+             dim3(kBlockThreads), static_cast<const T *>(grad), grad_stride, static_cast<const T *>(c.rows),       \
+             c.row_stride, c.places, c.kept, static_cast<const W *>(c.weights), static_cast<T *>(grad_rows),       \
+             static_cast<W *>(grad_weights), static_cast<uint32_t>(pairs), slots, c.choices, vectors,              \
+             static_cast<int>(c.D), magic, shift)
+  // (the narrowest group that holds a row; for rows of more than 256 vectors a workgroup: 16384 tokens, 4 rows of 512
+  // vectors each 232 us, a wavefront per row 250; for 256 vectors, 32768 tokens, 8 rows each, 463 and 447)
+  if (vectors <= 8) { TBE_COMBINE_BACKWARD(8); }
+  else if (vectors <= 16) { TBE_COMBINE_BACKWARD(16); }
+  else if (vectors <= 32) { TBE_COMBINE_BACKWARD(32); }
+  else if (vectors <= 256) { TBE_COMBINE_BACKWARD(64); }
+  else {
+    slots = ceil_div(c.tokens, kNumXcd) * kNumXcd * c.choices;
+    TBE_COMBINE_BACKWARD(256);
+  }
+#undef TBE_COMBINE_BACKWARD
 }
 
 template <typename T, typename W, int VEC>
 void launch_combine_backward(const CombineCall &c, const void *grad, int64_t grad_stride, void *grad_rows,
                              void *grad_weights) {
-  const int vectors = static_cast<int>(c.D / VEC);
-#define TBE_COMBINE_BACKWARD(GROUP)                                                                                \
-  TBE_LAUNCH("expert_combine_backward", c.stream, (expert_combine_backward_kernel<T, W, VEC, GROUP>),              \
-             dim3(static_cast<unsigned>(std::min(ceil_div(c.tokens, kBlockThreads / GROUP), kMaxGrid))), dim3(kBlockThreads), \
-             static_cast<const T *>(grad), grad_stride, static_cast<const T *>(c.rows), c.row_stride, c.places,    \
-             c.kept, static_cast<const W *>(c.weights), static_cast<T *>(grad_rows),                               \
-             static_cast<W *>(grad_weights), c.tokens, c.choices, vectors)
-  if (vectors <= 16) { TBE_COMBINE_BACKWARD(16); }
-  else if (vectors <= 256) { TBE_COMBINE_BACKWARD(64); }
-  else { TBE_COMBINE_BACKWARD(256); }
-#undef TBE_COMBINE_BACKWARD
+  if constexpr (VEC > 1) {
+    if (streams(c.tokens * c.choices, c.D * sizeof(T)))
+      return launch_combine_backward_as<T, W, VEC, true>(c, grad, grad_stride, grad_rows, grad_weights);
+  }
+  launch_combine_backward_as<T, W, VEC, false>(c, grad, grad_stride, grad_rows, grad_weights);
 }
 
-// f(T{}, W{}, VEC) for the types and the vector width of a call
-template <typename T, typename W, typename F> void with_vector(int bytes, F &&f) {
-  const int vec = bytes / static_cast<int>(sizeof(T));
-  if constexpr (sizeof(T) == 2) {
-    if (vec >= 8) return f(T{}, W{}, std::integral_constant<int, 8>{});
-  }
-  if constexpr (sizeof(T) <= 4) {
-    if (vec >= 4) return f(T{}, W{}, std::integral_constant<int, 4>{});
-  }
-  if (vec >= 2) return f(T{}, W{}, std::integral_constant<int, 2>{});
+// f(T{}, W{}, VEC) for the types of a call: 16-byte vectors, single elements for rows that hold no vector
+template <typename T, typename W, typename F> void with_vector(int64_t D, F &&f) {
+  constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+  if (D >= kVec) return f(T{}, W{}, std::integral_constant<int, kVec>{});
   return f(T{}, W{}, std::integral_constant<int, 1>{});
 }
-template <typename F> void with_types(int32_t dtype, int32_t weights_dtype, int bytes, F &&f) {
+template <typename F> void with_types(int32_t dtype, int32_t weights_dtype, int64_t D, F &&f) {
   const bool f32 = weights_dtype == TBE_DTYPE_F32;
   switch (dtype) {
-    case TBE_DTYPE_F32: return with_vector<float, float>(bytes, f);
-    case TBE_DTYPE_F16: return f32 ? with_vector<_Float16, float>(bytes, f) : with_vector<_Float16, _Float16>(bytes, f);
-    case TBE_DTYPE_BF16: return f32 ? with_vector<__bf16, float>(bytes, f) : with_vector<__bf16, __bf16>(bytes, f);
-    default: return f32 ? with_vector<double, float>(bytes, f) : with_vector<double, double>(bytes, f);
+    case TBE_DTYPE_F32: return with_vector<float, float>(D, f);
+    case TBE_DTYPE_F16: return f32 ? with_vector<_Float16, float>(D, f) : with_vector<_Float16, _Float16>(D, f);
+    case TBE_DTYPE_BF16: return f32 ? with_vector<__bf16, float>(D, f) : with_vector<__bf16, __bf16>(D, f);
+    default: return f32 ? with_vector<double, float>(D, f) : with_vector<double, double>(D, f);
   }
 }
+
+// (addresses need the alignment of an element, whatever the vectors')
+bool aligned(const void *p, int32_t dtype) { return address(p) % element_size(dtype) == 0; }
 
 int check_rows(const char *name, int32_t dtype, int64_t tokens, int32_t choices, int32_t experts, int64_t D) {
   TBE_REQUIRE(float_dtype(dtype), "%s: bad dtype %d", name, dtype);
@@ -532,7 +680,7 @@ extern "C" int tbe_expert_plan(const void *expert_ids, int32_t id_bytes, int64_t
               kMaxExperts, num_experts);
   TBE_REQUIRE(expert_offsets && (num_pairs == 0 || (expert_ids && order && places)), "%s: null pointer argument", name);
   const PlanRegions p = plan_regions(num_pairs, num_experts);
-  if (!workspace || workspace_bytes < p.total_bytes)
+  if (p.total_bytes > 0 && (!workspace || workspace_bytes < p.total_bytes))
     return fail(TBE_ERR_WORKSPACE, "%s: workspace of %llu bytes needed, %llu given", name,
                 (unsigned long long)p.total_bytes, (unsigned long long)workspace_bytes);
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -550,22 +698,23 @@ extern "C" int tbe_expert_dispatch(const void *tokens, int64_t token_stride, int
   TBE_REQUIRE(token_stride >= 0, "%s: token_stride must not be negative", name);
   if (num_tokens == 0) return TBE_OK;
   TBE_REQUIRE(tokens && places && expert_offsets && rows, "%s: null pointer argument", name);
-  const uint64_t size = element_size(dtype);
-  const int bytes = vector_bytes(D * size | token_stride * size | address(tokens) | address(rows));
-  TBE_REQUIRE(bytes >= static_cast<int>(size), "%s: misaligned pointer", name);
-  dim3 grid;
-  const RowTiles r = row_tiles(num_tokens, choices, D * size / bytes, &grid);
-  TBE_REQUIRE(grid.y <= 65535, "%s: D out of range", name);
-  const int64_t stride = token_stride * size / bytes;
+  TBE_REQUIRE(aligned(tokens, dtype) && aligned(rows, dtype), "%s: misaligned pointer", name);
+  const int64_t size = static_cast<int64_t>(element_size(dtype));
+  const int64_t row_bytes = D * size;
+  const int64_t unit = row_bytes >= 16 ? 16 : size;
+  const bool stream_out = streams(num_tokens * choices, row_bytes) && whole_lines(rows, row_bytes);
   const int32_t *kept = expert_offsets + num_experts;
   hipStream_t s = static_cast<hipStream_t>(stream);
-#define TBE_DISPATCH(U)                                                                                           \
-  TBE_LAUNCH("expert_dispatch", s, (expert_dispatch_kernel<U, kRowIter>), grid, dim3(kBlockThreads),              \
-             static_cast<const U *>(tokens), stride, places, kept, static_cast<U *>(rows), r)
-  if (bytes == 16) { TBE_DISPATCH(uint4); }
-  else if (bytes == 8) { TBE_DISPATCH(uint2); }
-  else if (bytes == 4) { TBE_DISPATCH(uint32_t); }
-  else { TBE_DISPATCH(uint16_t); }
+#define TBE_DISPATCH(U, STREAM)                                                                                   \
+  TBE_LAUNCH("expert_dispatch", s, (expert_dispatch_kernel<U, STREAM>), grid, dim3(kBlockThreads),                \
+             static_cast<const char *>(tokens), token_stride * size, places, kept, static_cast<char *>(rows), m)
+  for_row_maps(num_tokens, choices, ceil_div(row_bytes, unit), row_bytes, [&](const RowMap &m, dim3 grid) {
+    if (unit == 16 && stream_out) { TBE_DISPATCH(Words16, true); }
+    else if (unit == 16) { TBE_DISPATCH(Words16, false); }
+    else if (unit == 8) { TBE_DISPATCH(uint64_t, false); }
+    else if (unit == 4) { TBE_DISPATCH(uint32_t, false); }
+    else { TBE_DISPATCH(uint16_t, false); }
+  });
 #undef TBE_DISPATCH
   return check_launch(name);
 }
@@ -582,12 +731,10 @@ extern "C" int tbe_expert_combine(const void *rows, int64_t row_stride, int32_t 
               "%s: weights must be fp32 or of the rows' type", name);
   if (num_tokens == 0) return TBE_OK;
   TBE_REQUIRE(rows && places && expert_offsets && output, "%s: null pointer argument", name);
-  const uint64_t size = element_size(dtype);
-  const int bytes = vector_bytes(D * size | row_stride * size | address(rows) | address(output));
-  TBE_REQUIRE(bytes >= static_cast<int>(size), "%s: misaligned pointer", name);
+  TBE_REQUIRE(aligned(rows, dtype) && aligned(output, dtype), "%s: misaligned pointer", name);
   const CombineCall c{rows, row_stride, places, expert_offsets + num_experts, weights, num_tokens, choices, D,
                       static_cast<hipStream_t>(stream)};
-  with_types(dtype, weights ? weights_dtype : dtype, bytes, [&](auto t, auto w, auto vec) {
+  with_types(dtype, weights ? weights_dtype : dtype, D, [&](auto t, auto w, auto vec) {
     launch_combine<decltype(t), decltype(w), decltype(vec)::value>(c, output);
   });
   return check_launch(name);
@@ -608,13 +755,11 @@ extern "C" int tbe_expert_combine_backward(const void *grad_output, int64_t grad
   TBE_REQUIRE(grad_output && places && expert_offsets && weights && (rows || !grad_weights) &&
                   (grad_rows || grad_weights),
               "%s: null pointer argument", name);
-  const uint64_t size = element_size(dtype);
-  const int bytes = vector_bytes(D * size | row_stride * size | grad_stride * size | address(rows) |
-                                 address(grad_output) | address(grad_rows));
-  TBE_REQUIRE(bytes >= static_cast<int>(size), "%s: misaligned pointer", name);
+  TBE_REQUIRE(aligned(grad_output, dtype) && aligned(rows, dtype) && aligned(grad_rows, dtype),
+              "%s: misaligned pointer", name);
   const CombineCall c{rows, row_stride, places, expert_offsets + num_experts, weights, num_tokens, choices, D,
                       static_cast<hipStream_t>(stream)};
-  with_types(dtype, weights_dtype, bytes, [&](auto t, auto w, auto vec) {
+  with_types(dtype, weights_dtype, D, [&](auto t, auto w, auto vec) {
     launch_combine_backward<decltype(t), decltype(w), decltype(vec)::value>(c, grad_output, grad_stride, grad_rows,
                                                                           grad_weights);
   });

@@ -27,17 +27,18 @@ def test_plan_refusals():
     assert "num_experts" in _message(plan(experts=tbe_native.MAX_EXPERTS + 1))
     assert "null" in _message(plan(ids=NULL))
     assert "workspace" in _message(plan(pairs=100000, nbytes=16), code=2)
-    assert "workspace" in _message(plan(ws=NULL), code=2)
+    assert "workspace" in _message(plan(ws=NULL, pairs=100000), code=2)
 
 
 def test_plan_workspace_query():
     lib = tbe_native.load()
     size = lib.tbe_expert_plan_workspace_bytes
     assert size(-1, 4) == size(2 ** 31 - 1, 4) == size(4, 0) == size(4, tbe_native.MAX_EXPERTS + 1) == 0
-    assert size(0, 1) > 0
+    assert size(100000, 4) > 0
     # a workspace sized for a maximum serves every smaller batch
-    for experts in (1, 255, 256, 1024, 4095):
-        sizes = [size(n, experts) for n in (0, 1, 8192, 8193, 100000, 1 << 20, (1 << 31) - 2)]
+    for experts in (1, 60, 255, 256, 1023, 1024, 4095):
+        sizes = [size(n, experts) for n in (0, 1, 1024, 1025, 8193, 16384, 16385, 65536, 65537, 100000, 262144, 262145,
+                                              300000, 524288, 524289, 1 << 20, (1 << 31) - 2)]
         assert sizes == sorted(sizes)
 
 

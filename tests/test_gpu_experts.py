@@ -52,7 +52,9 @@ def make_ids(seed, tokens, choices, experts, drop=0.0, dtype=np.int64, same=Fals
 PLANS = [(1, 1, 1, 0.0), (1, 2, 8, 0.0), (63, 1, 7, 0.1), (64, 1, 2, 0.0), (65, 3, 5, 0.5), (1000, 8, 255, 0.0),
          (1024, 8, 256, 0.2), (4096, 2, 1023, 0.0), (4097, 2, 64, 0.1), (700, 3, 1024, 0.0), (2048, 1, 4095, 0.3),
          (683, 3, 4095, 0.0), (50001, 5, 60, 0.17), (40000, 8, 300, 0.0), (30011, 4, 2000, 0.05), (300, 2, 9, 1.0),
-         (9000, 1, 9, 1.0)]
+         (9000, 1, 9, 1.0), (1024, 1, 255, 0.1), (1025, 1, 255, 0.1), (512, 2, 1023, 0.1), (513, 2, 1023, 0.0),
+         (131072, 2, 200, 0.1), (131073, 2, 200, 0.1), (300001, 2, 100, 0.0), (65600, 8, 64, 0.1), (300000, 4, 3, 0.0),
+         (5000, 3, 4000, 0.1), (2500, 1, 4095, 0.0), (20000, 2, 1023, 0.2)]
 
 
 @pytest.mark.parametrize("tokens,choices,experts,drop", PLANS)
