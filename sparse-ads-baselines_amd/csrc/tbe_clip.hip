@@ -19,34 +19,46 @@ namespace tbe {
 namespace {
 
 // ------------------------------------------------------------------------------ lists of tensors
-// A launch takes up to kListTensors tensors of one type by kernel argument (under 4 KB).  A tensor is cut into
-// chunks of whole 16-byte vectors, counted from the 16-byte boundary at or before its first element: the
-// first and the last vector of a tensor may be partly outside it and are then taken element by element.
+// A launch takes up to kListTensors tensors of one type by kernel argument (under 4 KB), cut into chunks of
+// kChunkVectors 16-byte vectors; the elements behind a tensor's last whole vector are taken one by one.  The tensors
+// need no alignment: the memory system takes 16-byte accesses at any element's address.
 constexpr int kListTensors = 128;
+constexpr int kChunkVectors = 1024;  // 16 KB
 struct TensorList {
   const void *src[kListTensors];
   void *dst[kListTensors];
   int64_t numel[kListTensors];
-  int32_t chunk_end[kListTensors];  // running number of chunks
+  int32_t chunk_end[kListTensors];  // running number of chunks; INT32_MAX behind the last tensor
   int32_t count;
   int32_t chunks;
-  int32_t chunk_vectors;
 };
 
+// The tensor that a chunk belongs to: every lane looks at two of the ends.
 __device__ __forceinline__ int tensor_of_chunk(const TensorList &list, int chunk) {
-  int lo = 0, hi = list.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (chunk < list.chunk_end[mid]) hi = mid;
-    else lo = mid + 1;
-  }
-  return lo;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int before = __popcll(__ballot(list.chunk_end[lane] <= chunk)) +
+                     __popcll(__ballot(list.chunk_end[kWave + lane] <= chunk));
+  return __builtin_amdgcn_readfirstlane(before);
 }
 
-template <typename T> struct alignas(16) Vec16 {
-  static constexpr int kCount = 16 / sizeof(T);
-  T v[kCount];
+template <typename T> struct Piece {
+  const T *src;
+  T *dst;
+  int64_t first;  // of the chunk's elements, inside the tensor
+  int count;      // its elements
 };
+template <typename T> __device__ __forceinline__ Piece<T> piece_of_chunk(const TensorList &list, int chunk) {
+  constexpr int64_t kElements = kChunkVectors * (16 / sizeof(T));
+  const int t = tensor_of_chunk(list, chunk);
+  Piece<T> p;
+  p.src = static_cast<const T *>(list.src[t]);
+  p.dst = static_cast<T *>(list.dst[t]);
+  p.first = (chunk - (t ? list.chunk_end[t - 1] : 0)) * kElements;
+  p.count = static_cast<int>(min(kElements, list.numel[t] - p.first));
+  return p;
+}
+
+__device__ __forceinline__ double square(double x) { return x * x; }
 
 // What the lanes of this wavefront have written to LDS is there for its other lanes.
 __device__ __forceinline__ void wave_sync() {
@@ -60,115 +72,130 @@ __device__ __forceinline__ double wave_sum(double v) {
   for (int m = 1; m < kWave; m <<= 1) v += shfl_x(v, m);
   return v;
 }
-// Sum over the workgroup, in thread 0.
+// Sum over the workgroup, in every thread.
 template <int WAVES> __device__ __forceinline__ double block_sum(double v) {
   __shared__ double s_wave[WAVES];
   v = wave_sum(v);
   if ((threadIdx.x & (kWave - 1)) == 0) s_wave[threadIdx.x >> 6] = v;
   __syncthreads();
   double sum = 0.0;
-  if (threadIdx.x == 0) {
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) sum += s_wave[w];
-  }
+  for (int w = 0; w < WAVES; ++w) sum += s_wave[w];
   return sum;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kBlockThreads) void square_sum_kernel(TensorList list, double *__restrict__ partial) {
-  using V = Vec16<T>;
+// This thread's squares of a chunk that THREADS threads share.
+template <typename T, int THREADS, bool STREAM>
+__device__ __forceinline__ double chunk_squares(const Piece<T> &p, int thread) {
+  constexpr int kVec = 16 / sizeof(T);
+  constexpr int kAhead = 4;
+  const T *src = p.src + p.first;
+  const int vectors = p.count / kVec;
   double sum = 0.0;
-  for (int chunk = blockIdx.x; chunk < list.chunks; chunk += gridDim.x) {
-    const int t = tensor_of_chunk(list, chunk);
-    const T *src = static_cast<const T *>(list.src[t]);
-    const int offset = static_cast<int>((reinterpret_cast<uint64_t>(src) & 15) / sizeof(T));
-    const V *base = reinterpret_cast<const V *>(src - offset);
-    const int64_t end = offset + list.numel[t];  // in elements from `base`
-    const int64_t first = static_cast<int64_t>(chunk - (t ? list.chunk_end[t - 1] : 0)) * list.chunk_vectors;
-    const int64_t last = min(first + list.chunk_vectors, (end + V::kCount - 1) / V::kCount);
-    for (int64_t i = first + threadIdx.x; i < last; i += kBlockThreads) {
-      if (i * V::kCount >= offset && (i + 1) * V::kCount <= end) {
-        const V x = base[i];
+  for (int i0 = thread; i0 < vectors; i0 += THREADS * kAhead) {
+    Pack<T, kVec> x[kAhead];
 #pragma unroll
-        for (int q = 0; q < V::kCount; ++q) {
-          const double d = static_cast<double>(x.v[q]);
-          sum += d * d;
-        }
-      } else {
-        const T *e = reinterpret_cast<const T *>(base + i);
+    for (int u = 0; u < kAhead; ++u) {
+      const int i = i0 + u * THREADS;
+      x[u] = load_pack<T, kVec, STREAM>(src + min(i, vectors - 1) * kVec);  // clamped: no branch per load
+    }
 #pragma unroll
-        for (int q = 0; q < V::kCount; ++q) {
-          const int64_t at = i * V::kCount + q;
-          if (at >= offset && at < end) {
-            const double d = static_cast<double>(e[q]);
-            sum += d * d;
-          }
-        }
-      }
+    for (int u = 0; u < kAhead; ++u) {
+      if (i0 + u * THREADS >= vectors) break;
+#pragma unroll
+      for (int q = 0; q < kVec; ++q) sum += square(static_cast<double>(x[u].v[q]));
     }
   }
+  const int rest = vectors * kVec + thread;
+  if (rest < p.count) sum += square(static_cast<double>(src[rest]));
+  return sum;
+}
+
+// dst = src * scale for a chunk that THREADS threads share: products in 32 bits for the types of up to 32, rounded
+// once more for those of 16.
+template <typename T, int THREADS, bool STREAM_IN, bool STREAM_OUT>
+__device__ __forceinline__ void chunk_scaled(const Piece<T> &p, typename AccOf<T>::type scale, int thread) {
+  using A = typename AccOf<T>::type;
+  constexpr int kVec = 16 / sizeof(T);
+  const T *src = p.src + p.first;
+  T *dst = p.dst + p.first;
+  const int vectors = p.count / kVec;
+  for (int i = thread; i < vectors; i += THREADS) {
+    Pack<T, kVec> x = load_pack<T, kVec, STREAM_IN>(src + i * kVec);
+#pragma unroll
+    for (int q = 0; q < kVec; ++q) x.v[q] = static_cast<T>(static_cast<A>(x.v[q]) * scale);
+    store_pack<T, kVec, STREAM_OUT>(dst + i * kVec, x);
+  }
+  const int rest = vectors * kVec + thread;
+  if (rest < p.count) dst[rest] = static_cast<T>(static_cast<A>(src[rest]) * scale);
+}
+
+__device__ __forceinline__ void store_norm(void *norm, int f64, double sum) {
+  if (f64) *static_cast<double *>(norm) = sqrt(sum);
+  else *static_cast<float *>(norm) = static_cast<float>(sqrt(sum));
+}
+
+// The norm is rounded once, to the type it is stored in; the scale is formed in 64 bits from it.
+__device__ __forceinline__ double clip_scale(double norm, double max_norm) {
+  const double scale = max_norm / (norm + 1e-6);
+  // (no limit: nothing is scaled, infinities included)
+  return scale > 1.0 || (isinf(max_norm) && isinf(norm)) ? 1.0 : scale;
+}
+
+// A grid that fills the chip once walks the chunks; a partial sum per workgroup.
+template <typename T, bool STREAM>
+__global__ __launch_bounds__(kBlockThreads) void square_sum_kernel(TensorList list, double *__restrict__ partial) {
+  double sum = 0.0;
+  for (int chunk = blockIdx.x; chunk < list.chunks; chunk += gridDim.x)
+    sum += chunk_squares<T, kBlockThreads, STREAM>(piece_of_chunk<T>(list, chunk), threadIdx.x);
   sum = block_sum<kWavesPerBlock>(sum);
   if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
 
-constexpr int kFinishThreads = 1024;
-__global__ __launch_bounds__(kFinishThreads) void norm_finish_kernel(const double *__restrict__ partial, int64_t count,
-                                                                    void *norm, int f64) {
+constexpr int kWideThreads = 1024;
+__global__ __launch_bounds__(kWideThreads) void norm_finish_kernel(const double *__restrict__ partial, int64_t count,
+                                                                  void *norm, int f64) {
   double sum = 0.0;
-  for (int64_t i = threadIdx.x; i < count; i += kFinishThreads) sum += partial[i];
-  sum = block_sum<kFinishThreads / kWave>(sum);
-  if (threadIdx.x == 0) {
-    if (f64) *static_cast<double *>(norm) = sqrt(sum);
-    else *static_cast<float *>(norm) = static_cast<float>(sqrt(sum));
+  for (int64_t i = threadIdx.x; i < count; i += kWideThreads) sum += partial[i];
+  sum = block_sum<kWideThreads / kWave>(sum);
+  if (threadIdx.x == 0) store_norm(norm, f64, sum);
+}
+
+// A workgroup per chunk, a vector per thread: a copy of 1.2 GB took 381 us that way, 469 us with a grid that fills the
+// chip once and walks the chunks, 427 us with four vectors a thread (reading and writing want many short requests).
+template <typename T, bool STREAM_IN, bool STREAM_OUT>
+__global__ __launch_bounds__(kWideThreads) void scale_kernel(TensorList list, const void *norm, int f64, double max_norm) {
+  using A = typename AccOf<T>::type;
+  const double n = f64 ? *static_cast<const double *>(norm) : static_cast<double>(*static_cast<const float *>(norm));
+  const A scale = static_cast<A>(clip_scale(n, max_norm));
+  for (int chunk = blockIdx.x; chunk < list.chunks; chunk += gridDim.x) {
+    const Piece<T> p = piece_of_chunk<T>(list, chunk);
+    if (p.dst == p.src && scale == A(1)) continue;  // in place and within the limit: nothing changes
+    chunk_scaled<T, kWideThreads, STREAM_IN, STREAM_OUT>(p, scale, threadIdx.x);
   }
 }
 
-// The norm is rounded once, to the type it is stored in; the scale is formed in 64 bits from it.
-__device__ __forceinline__ double clip_scale(const void *norm, int f64, double max_norm) {
-  const double n = f64 ? *static_cast<const double *>(norm) : static_cast<double>(*static_cast<const float *>(norm));
-  const double scale = max_norm / (n + 1e-6);
-  // (no limit: nothing is scaled, infinities included)
-  return scale > 1.0 || (isinf(max_norm) && isinf(n)) ? 1.0 : scale;
-}
-
-// (products in 32 bits for the types of up to 32, rounded once more for those of 16)
+// Few chunks: norm and scaling in one workgroup, a wavefront per chunk.
+constexpr int kFewChunks = 32;
 template <typename T>
-__global__ __launch_bounds__(kBlockThreads) void scale_kernel(TensorList list, const void *norm, int f64, double max_norm) {
+__global__ __launch_bounds__(kWideThreads) void clip_few_kernel(TensorList list, int scaled, void *norm, int f64,
+                                                                double max_norm) {
   using A = typename AccOf<T>::type;
-  using V = Vec16<T>;
-  const A scale = static_cast<A>(clip_scale(norm, f64, max_norm));
-  for (int chunk = blockIdx.x; chunk < list.chunks; chunk += gridDim.x) {
-    const int t = tensor_of_chunk(list, chunk);
-    const T *src = static_cast<const T *>(list.src[t]);
-    T *dst = static_cast<T *>(list.dst[t]);
-    if (dst == src && scale == A(1)) continue;  // in place and within the limit: nothing changes
-    const int offset = static_cast<int>((reinterpret_cast<uint64_t>(src) & 15) / sizeof(T));
-    const bool together = ((reinterpret_cast<uint64_t>(src) ^ reinterpret_cast<uint64_t>(dst)) & 15) == 0;
-    const V *base = reinterpret_cast<const V *>(src - offset);
-    T *out = dst - offset;
-    const int64_t end = offset + list.numel[t];
-    const int64_t first = static_cast<int64_t>(chunk - (t ? list.chunk_end[t - 1] : 0)) * list.chunk_vectors;
-    const int64_t last = min(first + list.chunk_vectors, (end + V::kCount - 1) / V::kCount);
-    for (int64_t i = first + threadIdx.x; i < last; i += kBlockThreads) {
-      if (i * V::kCount >= offset && (i + 1) * V::kCount <= end) {
-        V x = base[i];
-#pragma unroll
-        for (int q = 0; q < V::kCount; ++q) x.v[q] = static_cast<T>(static_cast<A>(x.v[q]) * scale);
-        if (together) {
-          reinterpret_cast<V *>(out)[i] = x;
-        } else {
-#pragma unroll
-          for (int q = 0; q < V::kCount; ++q) out[i * V::kCount + q] = x.v[q];
-        }
-      } else {
-        const T *e = reinterpret_cast<const T *>(base + i);
-#pragma unroll
-        for (int q = 0; q < V::kCount; ++q) {
-          const int64_t at = i * V::kCount + q;
-          if (at >= offset && at < end) out[at] = static_cast<T>(static_cast<A>(e[q]) * scale);
-        }
-      }
-    }
+  constexpr int kWaves = kWideThreads / kWave;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = threadIdx.x >> 6;
+  double sum = 0.0;
+  for (int chunk = wave; chunk < list.chunks; chunk += kWaves)
+    sum += chunk_squares<T, kWave, false>(piece_of_chunk<T>(list, chunk), lane);
+  sum = block_sum<kWaves>(sum);
+  if (threadIdx.x == 0) store_norm(norm, f64, sum);
+  if (!scaled) return;
+  const double n = f64 ? sqrt(sum) : static_cast<double>(static_cast<float>(sqrt(sum)));
+  const A scale = static_cast<A>(clip_scale(n, max_norm));
+  for (int chunk = wave; chunk < list.chunks; chunk += kWaves) {
+    const Piece<T> p = piece_of_chunk<T>(list, chunk);
+    if (p.dst == p.src && scale == A(1)) continue;
+    chunk_scaled<T, kWave, false, false>(p, scale, lane);
   }
 }
 
@@ -368,38 +395,38 @@ __global__ __launch_bounds__(kBlockThreads) void table_norm_join_kernel(
 }
 
 // ------------------------------------------------------------------------------------------ host
-constexpr int kMaxBlocks = 256 * 8;   // of a launch over a list: eight workgroups per compute unit
+constexpr int kMaxBlocks = 256 * 8;   // of a sum over a list: eight workgroups per compute unit
+constexpr int kMaxGrid = 1 << 21;     // workgroups of a launch: grid times workgroup stays below 2^32 threads
 constexpr int kJoinBlocks = 1024;
 
 size_t size_of(int32_t dtype) { return dtype == TBE_DTYPE_F64 ? 8 : dtype == TBE_DTYPE_F32 ? 4 : 2; }
 
+int64_t chunks_of(int64_t numel, int32_t dtype) { return ceil_div(numel * static_cast<int64_t>(size_of(dtype)), kChunkVectors * 16); }
+
 // A list of one type, in pieces of kListTensors tensors.  f(list) is called for every piece.
 template <typename F>
 void for_lists(const void *const *src, void *const *dst, const int64_t *numel, const int32_t *dtypes, int32_t count,
-               int32_t dtype, int chunk_vectors, F &&f) {
+               int32_t dtype, F &&f) {
   TensorList list;
   list.count = 0;
   list.chunks = 0;
-  list.chunk_vectors = chunk_vectors;
+  const auto emit = [&] {
+    for (int i = list.count; i < kListTensors; ++i) list.chunk_end[i] = INT32_MAX;
+    f(list);
+    list.count = list.chunks = 0;
+  };
   for (int32_t i = 0; i < count; ++i) {
     if (dtypes[i] != dtype || numel[i] == 0) continue;
-    const uint64_t offset = reinterpret_cast<uint64_t>(src[i]) & 15;
-    const int64_t chunks = ceil_div(ceil_div(static_cast<int64_t>(offset + numel[i] * size_of(dtype)), 16), chunk_vectors);
-    if (list.count == kListTensors || list.chunks + chunks > INT32_MAX / 2) {
-      f(list);
-      list.count = list.chunks = 0;
-    }
+    const int64_t chunks = chunks_of(numel[i], dtype);
+    if (list.count == kListTensors || list.chunks + chunks > INT32_MAX / 2) emit();
     list.src[list.count] = src[i];
     list.dst[list.count] = dst ? dst[i] : nullptr;
     list.numel[list.count] = numel[i];
     list.chunks += static_cast<int32_t>(chunks);
     list.chunk_end[list.count++] = list.chunks;
   }
-  if (list.count) f(list);
+  if (list.count) emit();
 }
-
-// 16 KB a chunk
-constexpr int kChunkVectors = 1024;
 
 struct ListCall {
   const void *const *gradients;
@@ -458,45 +485,90 @@ int check_overlap(const char *name, const ListCall &c) {
   return TBE_OK;
 }
 
-unsigned list_grid(const TensorList &list) { return static_cast<unsigned>(std::min(list.chunks, kMaxBlocks)); }
-
 constexpr int32_t kDtypes[] = {TBE_DTYPE_F32, TBE_DTYPE_F16, TBE_DTYPE_BF16, TBE_DTYPE_F64};
 
 // (every type of a list starts pieces of its own, so there are at most this many)
 int64_t max_pieces(int32_t count) { return count / kListTensors + 4; }
 
+template <typename F> void with_type(int32_t dtype, F &&f) {
+  switch (dtype) {
+    case TBE_DTYPE_F32: return f(float{});
+    case TBE_DTYPE_F16: return f(_Float16{});
+    case TBE_DTYPE_BF16: return f(__bf16{});
+    default: return f(double{});
+  }
+}
+
+uint64_t total_bytes(const ListCall &c) {
+  uint64_t bytes = 0;
+  for (int32_t i = 0; i < c.count; ++i) bytes += static_cast<uint64_t>(c.numels[i]) * size_of(c.dtypes[i]);
+  return bytes;
+}
+// More than the 256 MB memory-side cache holds: the second pass finds little of what the first one read, so both are
+// streamed (1.2 GB squared and scaled: 558 us, 619 with plain accesses; 240 MB: 116 and 99 the other way round).
+bool streams(uint64_t bytes) { return bytes > (uint64_t{256} << 20); }
+
 void launch_norm(const ListCall &c, void *workspace, void *norm, int32_t norm_dtype, hipStream_t s) {
   double *partial = static_cast<double *>(workspace);
   int64_t used = 0;
+  const bool stream = streams(total_bytes(c));
   for (const int32_t dtype : kDtypes) {
-    for_lists(c.gradients, nullptr, c.numels, c.dtypes, c.count, dtype, kChunkVectors, [&](const TensorList &list) {
-      const dim3 grid(list_grid(list)), block(kBlockThreads);
-      switch (dtype) {
-        case TBE_DTYPE_F32: TBE_LAUNCH("gradient_squares", s, square_sum_kernel<float>, grid, block, list, partial + used); break;
-        case TBE_DTYPE_F16: TBE_LAUNCH("gradient_squares", s, square_sum_kernel<_Float16>, grid, block, list, partial + used); break;
-        case TBE_DTYPE_BF16: TBE_LAUNCH("gradient_squares", s, square_sum_kernel<__bf16>, grid, block, list, partial + used); break;
-        default: TBE_LAUNCH("gradient_squares", s, square_sum_kernel<double>, grid, block, list, partial + used); break;
-      }
+    for_lists(c.gradients, nullptr, c.numels, c.dtypes, c.count, dtype, [&](const TensorList &list) {
+      const dim3 grid(static_cast<unsigned>(std::min(list.chunks, kMaxBlocks))), block(kBlockThreads);
+      with_type(dtype, [&](auto t) {
+        using T = decltype(t);
+        if (stream) TBE_LAUNCH("gradient_squares", s, (square_sum_kernel<T, true>), grid, block, list, partial + used);
+        else TBE_LAUNCH("gradient_squares", s, (square_sum_kernel<T, false>), grid, block, list, partial + used);
+      });
       used += grid.x;
     });
   }
-  TBE_LAUNCH("gradient_norm", s, norm_finish_kernel, dim3(1), dim3(kFinishThreads), partial, used, norm,
+  TBE_LAUNCH("gradient_norm", s, norm_finish_kernel, dim3(1), dim3(kWideThreads), partial, used, norm,
              norm_dtype == TBE_DTYPE_F64 ? 1 : 0);
 }
 
 void launch_scale(const ListCall &c, double max_norm, const void *norm, int32_t norm_dtype, hipStream_t s) {
   const int f64 = norm_dtype == TBE_DTYPE_F64 ? 1 : 0;
+  const uint64_t bytes = total_bytes(c);
+  // Outputs of their own push what the norm's pass has left out of the caches, unless they are streamed (240 MB: 63 us
+  // a pass, 85 with plain stores); small ones are left to whoever reads them next.
+  bool apart = false;
+  for (int32_t i = 0; i < c.count; ++i) apart = apart || (c.numels[i] && c.outputs[i] != c.gradients[i]);
+  const bool stream_in = streams(bytes), stream_out = stream_in || (apart && bytes > (uint64_t{32} << 20));
   for (const int32_t dtype : kDtypes) {
-    for_lists(c.gradients, c.outputs, c.numels, c.dtypes, c.count, dtype, kChunkVectors, [&](const TensorList &list) {
-      const dim3 grid(list_grid(list)), block(kBlockThreads);
-      switch (dtype) {
-        case TBE_DTYPE_F32: TBE_LAUNCH("gradient_scale", s, scale_kernel<float>, grid, block, list, norm, f64, max_norm); break;
-        case TBE_DTYPE_F16: TBE_LAUNCH("gradient_scale", s, scale_kernel<_Float16>, grid, block, list, norm, f64, max_norm); break;
-        case TBE_DTYPE_BF16: TBE_LAUNCH("gradient_scale", s, scale_kernel<__bf16>, grid, block, list, norm, f64, max_norm); break;
-        default: TBE_LAUNCH("gradient_scale", s, scale_kernel<double>, grid, block, list, norm, f64, max_norm); break;
-      }
+    for_lists(c.gradients, c.outputs, c.numels, c.dtypes, c.count, dtype, [&](const TensorList &list) {
+      const dim3 grid(static_cast<unsigned>(std::min(list.chunks, kMaxGrid))), block(kWideThreads);
+      with_type(dtype, [&](auto t) {
+        using T = decltype(t);
+        if (stream_in) TBE_LAUNCH("gradient_scale", s, (scale_kernel<T, true, true>), grid, block, list, norm, f64, max_norm);
+        else if (stream_out) TBE_LAUNCH("gradient_scale", s, (scale_kernel<T, false, true>), grid, block, list, norm, f64, max_norm);
+        else TBE_LAUNCH("gradient_scale", s, (scale_kernel<T, false, false>), grid, block, list, norm, f64, max_norm);
+      });
     });
   }
+}
+
+// A list of one type and few chunks goes through one workgroup in one launch: whether it did.  (Eleven fp32 tensors of
+// 60001 elements in all, 26 chunks.)
+bool launch_few(const ListCall &c, double max_norm, void *norm, int32_t norm_dtype, hipStream_t s) {
+  int32_t dtype = -1;
+  int64_t tensors = 0, chunks = 0;
+  for (int32_t i = 0; i < c.count; ++i) {
+    if (c.numels[i] == 0) continue;
+    if (dtype >= 0 && c.dtypes[i] != dtype) return false;
+    dtype = c.dtypes[i];
+    ++tensors;
+    chunks += chunks_of(c.numels[i], dtype);
+    if (tensors > kListTensors || chunks > kFewChunks) return false;
+  }
+  if (tensors == 0) return false;
+  for_lists(c.gradients, c.outputs, c.numels, c.dtypes, c.count, dtype, [&](const TensorList &list) {
+    with_type(dtype, [&](auto t) {
+      TBE_LAUNCH("gradient_clip_few", s, (clip_few_kernel<decltype(t)>), dim3(1), dim3(kWideThreads), list,
+                 c.outputs ? 1 : 0, norm, norm_dtype == TBE_DTYPE_F64 ? 1 : 0, max_norm);
+    });
+  });
+  return true;
 }
 
 int check_norm(const char *name, const void *norm, int32_t norm_dtype) {
@@ -557,7 +629,8 @@ extern "C" int tbe_gradient_norm(const void *const *gradients, const int64_t *nu
   if (int rc = check_list(name, c, false)) return rc;
   if (int rc = check_norm(name, norm, norm_dtype)) return rc;
   if (int rc = check_workspace(name, num_tensors, workspace, workspace_bytes)) return rc;
-  launch_norm(c, workspace, norm, norm_dtype, static_cast<hipStream_t>(stream));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (!launch_few(c, 0.0, norm, norm_dtype, s)) launch_norm(c, workspace, norm, norm_dtype, s);
   return check_launch(name);
 }
 
@@ -587,8 +660,10 @@ extern "C" int tbe_clip_gradients(const void *const *gradients, void *const *out
   if (int rc = check_workspace(name, num_tensors, workspace, workspace_bytes)) return rc;
   if (int rc = check_overlap(name, c)) return rc;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  launch_norm(c, workspace, norm, norm_dtype, s);
-  launch_scale(c, max_norm, norm, norm_dtype, s);
+  if (!launch_few(c, max_norm, norm, norm_dtype, s)) {
+    launch_norm(c, workspace, norm, norm_dtype, s);
+    launch_scale(c, max_norm, norm, norm_dtype, s);
+  }
   return check_launch(name);
 }
 
@@ -607,7 +682,7 @@ extern "C" int tbe_table_gradient_norm(const void *grad_output, int32_t dtype, i
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int f64 = norm_dtype == TBE_DTYPE_F64 ? 1 : 0;
   if (num_indices == 0) {
-    TBE_LAUNCH("gradient_norm", s, norm_finish_kernel, dim3(1), dim3(kFinishThreads), nullptr, int64_t{0}, norm, f64);
+    TBE_LAUNCH("gradient_norm", s, norm_finish_kernel, dim3(1), dim3(kWideThreads), nullptr, int64_t{0}, norm, f64);
     return check_launch(name);
   }
   tbe_workspace_layout_t l;
@@ -647,7 +722,7 @@ extern "C" int tbe_table_gradient_norm(const void *grad_output, int32_t dtype, i
       break;
     default: parts = launch_table<double, 2>(c, tiles, static_cast<int>(column_blocks)); break;
   }
-  TBE_LAUNCH("gradient_norm", s, norm_finish_kernel, dim3(1), dim3(kFinishThreads), c.partial,
+  TBE_LAUNCH("gradient_norm", s, norm_finish_kernel, dim3(1), dim3(kWideThreads), c.partial,
              static_cast<int64_t>(parts), norm, f64);
   return check_launch(name);
 }

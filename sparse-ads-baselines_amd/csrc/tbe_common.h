@@ -260,6 +260,37 @@ template <> __device__ __forceinline__ float from_acc<float, float>(float x) { r
 template <> __device__ __forceinline__ __half from_acc<__half, float>(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ double from_acc<double, double>(double x) { return x; }
 
+// Rows and lists of elements of any alignment: 16 bytes (VEC elements) at the address of any element of at least two
+// bytes, or single elements (VEC = 1).  STREAM: the data is touched once, and more than the caches hold.
+typedef uint32_t Words16 __attribute__((ext_vector_type(4), aligned(2)));
+
+template <typename T, int VEC> struct Pack {
+  T v[VEC];
+};
+template <typename T, int VEC, bool STREAM>
+__device__ __forceinline__ Pack<T, VEC> load_pack(const T *p) {
+  if constexpr (VEC == 1) {
+    return Pack<T, VEC>{{*p}};
+  } else {
+    static_assert(sizeof(Pack<T, VEC>) == 16, "full vectors");
+    const Words16 *w = reinterpret_cast<const Words16 *>(p);
+    Words16 x;
+    if constexpr (STREAM) x = __builtin_nontemporal_load(w);
+    else x = *w;
+    return __builtin_bit_cast(Pack<T, VEC>, x);
+  }
+}
+template <typename T, int VEC, bool STREAM>
+__device__ __forceinline__ void store_pack(T *p, const Pack<T, VEC> &v) {
+  if constexpr (VEC == 1) {
+    *p = v.v[0];
+  } else {
+    Words16 *w = reinterpret_cast<Words16 *>(p);
+    if constexpr (STREAM) __builtin_nontemporal_store(__builtin_bit_cast(Words16, v), w);
+    else *w = __builtin_bit_cast(Words16, v);
+  }
+}
+
 __device__ __forceinline__ float shfl_idx(float v, int src) { return __shfl(v, src, kWave); }
 __device__ __forceinline__ int shfl_idx(int v, int src) { return __shfl(v, src, kWave); }
 __device__ __forceinline__ double shfl_idx(double v, int src) { return __shfl(v, src, kWave); }

@@ -238,36 +238,6 @@ struct RowMap {
   int32_t shift;
 };
 
-// 16 bytes at the address of any 2-byte element
-typedef uint32_t Words16 __attribute__((ext_vector_type(4), aligned(2)));
-
-template <typename T, int VEC> struct Pack {
-  T v[VEC];
-};
-template <typename T, int VEC, bool STREAM>
-__device__ __forceinline__ Pack<T, VEC> load_pack(const T *p) {
-  if constexpr (VEC == 1) {
-    return Pack<T, VEC>{{*p}};
-  } else {
-    static_assert(sizeof(Pack<T, VEC>) == 16, "full vectors");
-    const Words16 *w = reinterpret_cast<const Words16 *>(p);
-    Words16 x;
-    if constexpr (STREAM) x = __builtin_nontemporal_load(w);
-    else x = *w;
-    return __builtin_bit_cast(Pack<T, VEC>, x);
-  }
-}
-template <typename T, int VEC, bool STREAM>
-__device__ __forceinline__ void store_pack(T *p, const Pack<T, VEC> &v) {
-  if constexpr (VEC == 1) {
-    *p = v.v[0];
-  } else {
-    Words16 *w = reinterpret_cast<Words16 *>(p);
-    if constexpr (STREAM) __builtin_nontemporal_store(__builtin_bit_cast(Words16, v), w);
-    else *w = __builtin_bit_cast(Words16, v);
-  }
-}
-
 // A dropped pair's place lies behind the rows kept; so do places that are none.
 __device__ __forceinline__ bool is_kept(int32_t place, int32_t kept) {
   return static_cast<uint32_t>(place) < static_cast<uint32_t>(kept);
