@@ -10,7 +10,7 @@
 
 #include <algorithm>
 #include <new>
-#include <utility>
+#include <type_traits>
 #include <vector>
 
 #include "tbe_stages.h"
@@ -19,42 +19,68 @@ namespace tbe {
 namespace {
 
 // ------------------------------------------------------------------------------ lists of tensors
-// A launch takes up to kListTensors tensors of one type by kernel argument (under 4 KB), cut into chunks of
-// kChunkVectors 16-byte vectors; the elements behind a tensor's last whole vector are taken one by one.  The tensors
-// need no alignment: the memory system takes 16-byte accesses at any element's address.
-constexpr int kListTensors = 128;
+// A launch takes a list of tensors of one type by kernel argument (under 4 KB), cut into chunks of kChunkVectors
+// 16-byte vectors.  Chunks begin at the first 16-byte boundary of the tensor that is written (read, for a sum): the
+// elements before it, fewer than a vector, belong to the first chunk, those behind the last whole vector to the
+// last one.  The other tensor of a pair may lie at any element's address, which the memory system takes.
+// An entry is 12 bytes (20 with an output of its own), so that 300 tensors take one launch a pass.
 constexpr int kChunkVectors = 1024;  // 16 KB
-struct TensorList {
-  const void *src[kListTensors];
-  void *dst[kListTensors];
-  int64_t numel[kListTensors];
-  int32_t chunk_end[kListTensors];  // running number of chunks; INT32_MAX behind the last tensor
-  int32_t count;
+constexpr int kListTensors = 320;    // read, or scaled in place
+constexpr int kPairTensors = 192;    // with outputs of their own
+constexpr int kNoBoundary = 0x8000;
+template <int N, bool PAIRS> struct TensorList {
+  static constexpr int kTensors = N;
+  static constexpr bool kPairs = PAIRS;
+  uint64_t src[N];                  // address, and above its 48 bits the last chunk's `count`, or kNoBoundary | elements
+  uint64_t dst[PAIRS ? N : 1];
+  int32_t chunk_end[N];             // running number of chunks; INT32_MAX behind the last tensor
   int32_t chunks;
 };
+using ReadList = TensorList<kListTensors, false>;
+using PairList = TensorList<kPairTensors, true>;
+static_assert(sizeof(ReadList) < 3900 && sizeof(PairList) < 3900, "kernel arguments");
 
-// The tensor that a chunk belongs to: every lane looks at two of the ends.
-__device__ __forceinline__ int tensor_of_chunk(const TensorList &list, int chunk) {
+// The tensor that a chunk belongs to: every lane looks at some of the ends.
+template <typename L> __device__ __forceinline__ int tensor_of_chunk(const L &list, int chunk) {
   const int lane = threadIdx.x & (kWave - 1);
-  const int before = __popcll(__ballot(list.chunk_end[lane] <= chunk)) +
-                     __popcll(__ballot(list.chunk_end[kWave + lane] <= chunk));
+  int before = 0;
+#pragma unroll
+  for (int i = 0; i < L::kTensors; i += kWave) before += __popcll(__ballot(list.chunk_end[i + lane] <= chunk));
   return __builtin_amdgcn_readfirstlane(before);
 }
 
 template <typename T> struct Piece {
-  const T *src;
+  const T *src;   // of the chunk's first vector
   T *dst;
-  int64_t first;  // of the chunk's elements, inside the tensor
-  int count;      // its elements
+  int count;      // elements from there on
+  int head;       // elements before it that belong to the chunk
 };
-template <typename T> __device__ __forceinline__ Piece<T> piece_of_chunk(const TensorList &list, int chunk) {
-  constexpr int64_t kElements = kChunkVectors * (16 / sizeof(T));
+// (elements before the first 16-byte boundary)
+template <typename T> __host__ __device__ __forceinline__ int head_of(uint64_t address) {
+  return static_cast<int>(((16 - (address & 15)) & 15) / sizeof(T));
+}
+template <typename T, typename L> __device__ __forceinline__ Piece<T> piece_of_chunk(const L &list, int chunk) {
+  constexpr int kElements = kChunkVectors * (16 / static_cast<int>(sizeof(T)));
   const int t = tensor_of_chunk(list, chunk);
+  const uint64_t packed = list.src[t];
+  const uint64_t src = packed & ((uint64_t{1} << 48) - 1);
+  const uint64_t dst = L::kPairs ? list.dst[L::kPairs ? t : 0] : src;
+  const int in_tensor = chunk - (t ? list.chunk_end[t - 1] : 0);
+  const int last = static_cast<int>(packed >> 48);
   Piece<T> p;
-  p.src = static_cast<const T *>(list.src[t]);
-  p.dst = static_cast<T *>(list.dst[t]);
-  p.first = (chunk - (t ? list.chunk_end[t - 1] : 0)) * kElements;
-  p.count = static_cast<int>(min(kElements, list.numel[t] - p.first));
+  int64_t first;
+  if (last & kNoBoundary) {  // the whole tensor lies before the boundary
+    p.head = last & ~kNoBoundary;
+    p.count = 0;
+    first = p.head;
+  } else {
+    const int head = head_of<T>(dst);
+    p.head = in_tensor == 0 ? head : 0;
+    p.count = chunk + 1 == list.chunk_end[t] ? last : kElements;
+    first = head + static_cast<int64_t>(in_tensor) * kElements;
+  }
+  p.src = reinterpret_cast<const T *>(src) + first;
+  p.dst = reinterpret_cast<T *>(dst) + first;
   return p;
 }
 
@@ -89,7 +115,7 @@ template <typename T, int THREADS, bool STREAM>
 __device__ __forceinline__ double chunk_squares(const Piece<T> &p, int thread) {
   constexpr int kVec = 16 / sizeof(T);
   constexpr int kAhead = 4;
-  const T *src = p.src + p.first;
+  const T *src = p.src;
   const int vectors = p.count / kVec;
   double sum = 0.0;
   for (int i0 = thread; i0 < vectors; i0 += THREADS * kAhead) {
@@ -108,6 +134,7 @@ __device__ __forceinline__ double chunk_squares(const Piece<T> &p, int thread) {
   }
   const int rest = vectors * kVec + thread;
   if (rest < p.count) sum += square(static_cast<double>(src[rest]));
+  if (thread < p.head) sum += square(static_cast<double>(src[thread - p.head]));
   return sum;
 }
 
@@ -117,8 +144,8 @@ template <typename T, int THREADS, bool STREAM_IN, bool STREAM_OUT>
 __device__ __forceinline__ void chunk_scaled(const Piece<T> &p, typename AccOf<T>::type scale, int thread) {
   using A = typename AccOf<T>::type;
   constexpr int kVec = 16 / sizeof(T);
-  const T *src = p.src + p.first;
-  T *dst = p.dst + p.first;
+  const T *src = p.src;
+  T *dst = p.dst;
   const int vectors = p.count / kVec;
   for (int i = thread; i < vectors; i += THREADS) {
     Pack<T, kVec> x = load_pack<T, kVec, STREAM_IN>(src + i * kVec);
@@ -128,6 +155,7 @@ __device__ __forceinline__ void chunk_scaled(const Piece<T> &p, typename AccOf<T
   }
   const int rest = vectors * kVec + thread;
   if (rest < p.count) dst[rest] = static_cast<T>(static_cast<A>(src[rest]) * scale);
+  if (thread < p.head) dst[thread - p.head] = static_cast<T>(static_cast<A>(src[thread - p.head]) * scale);
 }
 
 __device__ __forceinline__ void store_norm(void *norm, int f64, double sum) {
@@ -144,7 +172,7 @@ __device__ __forceinline__ double clip_scale(double norm, double max_norm) {
 
 // A grid that fills the chip once walks the chunks; a partial sum per workgroup.
 template <typename T, bool STREAM>
-__global__ __launch_bounds__(kBlockThreads) void square_sum_kernel(TensorList list, double *__restrict__ partial) {
+__global__ __launch_bounds__(kBlockThreads) void square_sum_kernel(ReadList list, double *__restrict__ partial) {
   double sum = 0.0;
   for (int chunk = blockIdx.x; chunk < list.chunks; chunk += gridDim.x)
     sum += chunk_squares<T, kBlockThreads, STREAM>(piece_of_chunk<T>(list, chunk), threadIdx.x);
@@ -161,24 +189,24 @@ __global__ __launch_bounds__(kWideThreads) void norm_finish_kernel(const double 
   if (threadIdx.x == 0) store_norm(norm, f64, sum);
 }
 
-// A workgroup per chunk, a vector per thread: a copy of 1.2 GB took 381 us that way, 469 us with a grid that fills the
-// chip once and walks the chunks, 427 us with four vectors a thread (reading and writing want many short requests).
-template <typename T, bool STREAM_IN, bool STREAM_OUT>
-__global__ __launch_bounds__(kWideThreads) void scale_kernel(TensorList list, const void *norm, int f64, double max_norm) {
+// A vector per thread and chunk (reading and writing want many short requests: 427 us with four vectors a thread where
+// this takes 381, a copy of 1.2 GB), a workgroup walking every kScaleBlocks-th chunk.  The grid is what a call within the
+// limit pays for, in place: 600 M bf16 elements take 194 us with up to 16384 workgroups, 246 with one per chunk, 177 for
+// the norm alone; scaled they take 572 either way, 592 with 2048 workgroups.
+template <typename T, typename L, bool STREAM_IN, bool STREAM_OUT>
+__global__ __launch_bounds__(kWideThreads) void scale_kernel(L list, const void *norm, int f64, double max_norm) {
   using A = typename AccOf<T>::type;
   const double n = f64 ? *static_cast<const double *>(norm) : static_cast<double>(*static_cast<const float *>(norm));
   const A scale = static_cast<A>(clip_scale(n, max_norm));
-  for (int chunk = blockIdx.x; chunk < list.chunks; chunk += gridDim.x) {
-    const Piece<T> p = piece_of_chunk<T>(list, chunk);
-    if (p.dst == p.src && scale == A(1)) continue;  // in place and within the limit: nothing changes
-    chunk_scaled<T, kWideThreads, STREAM_IN, STREAM_OUT>(p, scale, threadIdx.x);
-  }
+  if (!L::kPairs && scale == A(1)) return;  // in place and within the limit: nothing changes
+  for (int chunk = blockIdx.x; chunk < list.chunks; chunk += gridDim.x)
+    chunk_scaled<T, kWideThreads, STREAM_IN, STREAM_OUT>(piece_of_chunk<T>(list, chunk), scale, threadIdx.x);
 }
 
 // Few chunks: norm and scaling in one workgroup, a wavefront per chunk.
 constexpr int kFewChunks = 32;
-template <typename T>
-__global__ __launch_bounds__(kWideThreads) void clip_few_kernel(TensorList list, int scaled, void *norm, int f64,
+template <typename T, typename L>
+__global__ __launch_bounds__(kWideThreads) void clip_few_kernel(L list, int scaled, void *norm, int f64,
                                                                 double max_norm) {
   using A = typename AccOf<T>::type;
   constexpr int kWaves = kWideThreads / kWave;
@@ -192,11 +220,9 @@ __global__ __launch_bounds__(kWideThreads) void clip_few_kernel(TensorList list,
   if (!scaled) return;
   const double n = f64 ? sqrt(sum) : static_cast<double>(static_cast<float>(sqrt(sum)));
   const A scale = static_cast<A>(clip_scale(n, max_norm));
-  for (int chunk = wave; chunk < list.chunks; chunk += kWaves) {
-    const Piece<T> p = piece_of_chunk<T>(list, chunk);
-    if (p.dst == p.src && scale == A(1)) continue;
-    chunk_scaled<T, kWave, false, false>(p, scale, lane);
-  }
+  if (!L::kPairs && scale == A(1)) return;
+  for (int chunk = wave; chunk < list.chunks; chunk += kWaves)
+    chunk_scaled<T, kWave, false, false>(piece_of_chunk<T>(list, chunk), scale, lane);
 }
 
 // --------------------------------------------------------------------- norm of the tables' gradient
@@ -213,7 +239,8 @@ template <typename T, int VEC, bool WEIGHTED>
 __global__ __launch_bounds__(kBlockThreads) void table_norm_tiles_kernel(
     const T *__restrict__ grad, const T *__restrict__ psw, const int32_t *__restrict__ positions_sorted,
     const int32_t *__restrict__ grad_rows, const int32_t *__restrict__ segment_ids, int64_t n, int D,
-    int64_t num_tiles, typename AccOf<T>::type *__restrict__ partial_rows, double *__restrict__ tile_sums) {
+    int64_t num_tiles, int64_t blocks_per_xcd, typename AccOf<T>::type *__restrict__ partial_rows,
+    double *__restrict__ tile_sums) {
   using V = RowVec<T, VEC>;
   using A = typename V::A;
   using R = typename V::R;
@@ -225,7 +252,8 @@ __global__ __launch_bounds__(kBlockThreads) void table_norm_tiles_kernel(
   __shared__ A s_tail[kWavesPerBlock][kWave][VEC];
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = threadIdx.x >> 6;
-  const int64_t tile = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + wave;
+  // (the workgroups of an XCD walk one eighth of the sorted positions, so that a table's gradient rows stay in its L2)
+  const int64_t tile = xcd_contiguous(blockIdx.x, blocks_per_xcd) * kWavesPerBlock + wave;
   if (tile >= num_tiles) return;
   const int64_t p0 = tile * kTile;
   const int len = static_cast<int>(min(n - p0, static_cast<int64_t>(kTile)));
@@ -396,37 +424,10 @@ __global__ __launch_bounds__(kBlockThreads) void table_norm_join_kernel(
 
 // ------------------------------------------------------------------------------------------ host
 constexpr int kMaxBlocks = 256 * 8;   // of a sum over a list: eight workgroups per compute unit
-constexpr int kMaxGrid = 1 << 21;     // workgroups of a launch: grid times workgroup stays below 2^32 threads
+constexpr int kScaleBlocks = 1 << 14; // of a scaling launch (see scale_kernel)
 constexpr int kJoinBlocks = 1024;
 
 size_t size_of(int32_t dtype) { return dtype == TBE_DTYPE_F64 ? 8 : dtype == TBE_DTYPE_F32 ? 4 : 2; }
-
-int64_t chunks_of(int64_t numel, int32_t dtype) { return ceil_div(numel * static_cast<int64_t>(size_of(dtype)), kChunkVectors * 16); }
-
-// A list of one type, in pieces of kListTensors tensors.  f(list) is called for every piece.
-template <typename F>
-void for_lists(const void *const *src, void *const *dst, const int64_t *numel, const int32_t *dtypes, int32_t count,
-               int32_t dtype, F &&f) {
-  TensorList list;
-  list.count = 0;
-  list.chunks = 0;
-  const auto emit = [&] {
-    for (int i = list.count; i < kListTensors; ++i) list.chunk_end[i] = INT32_MAX;
-    f(list);
-    list.count = list.chunks = 0;
-  };
-  for (int32_t i = 0; i < count; ++i) {
-    if (dtypes[i] != dtype || numel[i] == 0) continue;
-    const int64_t chunks = chunks_of(numel[i], dtype);
-    if (list.count == kListTensors || list.chunks + chunks > INT32_MAX / 2) emit();
-    list.src[list.count] = src[i];
-    list.dst[list.count] = dst ? dst[i] : nullptr;
-    list.numel[list.count] = numel[i];
-    list.chunks += static_cast<int32_t>(chunks);
-    list.chunk_end[list.count++] = list.chunks;
-  }
-  if (list.count) emit();
-}
 
 struct ListCall {
   const void *const *gradients;
@@ -435,6 +436,53 @@ struct ListCall {
   const int32_t *dtypes;
   int32_t count;
 };
+
+// Chunks of a tensor whose boundaries are those of `address`, and what its last one holds.
+struct Chunks {
+  int64_t count;
+  int last;
+};
+Chunks chunks_of(int64_t numel, uint64_t address, int32_t dtype) {
+  const int64_t size = static_cast<int64_t>(size_of(dtype));
+  const int64_t head = static_cast<int64_t>((16 - (address & 15)) & 15) / size;
+  const int64_t elements = kChunkVectors * 16 / size;
+  if (numel < head) return Chunks{1, kNoBoundary | static_cast<int>(numel)};
+  const int64_t count = std::max<int64_t>(1, ceil_div(numel - head, elements));
+  return Chunks{count, static_cast<int>(numel - head - (count - 1) * elements)};
+}
+
+bool in_place(const ListCall &c) {
+  for (int32_t i = 0; i < c.count; ++i)
+    if (c.numels[i] && c.outputs[i] != c.gradients[i]) return false;
+  return true;
+}
+
+// A call's tensors of one type, in lists of at most L::kTensors.  f(list) is called for every one.
+template <typename L, typename F> void for_lists(const ListCall &c, int32_t dtype, F &&f) {
+  L list;
+  int tensors = 0;
+  list.chunks = 0;
+  const auto emit = [&] {
+    for (int i = tensors; i < L::kTensors; ++i) {
+      list.chunk_end[i] = INT32_MAX;
+      list.src[i] = 0;
+    }
+    f(list);
+    tensors = list.chunks = 0;
+  };
+  for (int32_t i = 0; i < c.count; ++i) {
+    if (c.dtypes[i] != dtype || c.numels[i] == 0) continue;
+    const uint64_t src = reinterpret_cast<uint64_t>(c.gradients[i]);
+    const uint64_t written = L::kPairs ? reinterpret_cast<uint64_t>(c.outputs[i]) : src;
+    const Chunks chunks = chunks_of(c.numels[i], written, dtype);
+    if (tensors == L::kTensors || list.chunks + chunks.count > INT32_MAX / 2) emit();
+    list.src[tensors] = src | static_cast<uint64_t>(chunks.last) << 48;
+    if constexpr (L::kPairs) list.dst[tensors] = written;
+    list.chunks += static_cast<int32_t>(chunks.count);
+    list.chunk_end[tensors++] = list.chunks;
+  }
+  if (tensors) emit();
+}
 
 int check_list(const char *name, const ListCall &c, bool outputs) {
   TBE_REQUIRE(c.count >= 0, "%s: num_tensors must not be negative", name);
@@ -446,6 +494,7 @@ int check_list(const char *name, const ListCall &c, bool outputs) {
     TBE_REQUIRE(c.numels[i] >= 0 && c.numels[i] <= (int64_t{1} << 40), "%s: element count of tensor %d out of range", name, i);
     if (c.numels[i] == 0) continue;
     TBE_REQUIRE(c.gradients[i] && (!outputs || c.outputs[i]), "%s: null pointer argument", name);
+    TBE_REQUIRE((reinterpret_cast<uint64_t>(c.gradients[i]) >> 48) == 0, "%s: address of tensor %d out of range", name, i);
     TBE_REQUIRE(reinterpret_cast<uint64_t>(c.gradients[i]) % size == 0 &&
                     (!outputs || reinterpret_cast<uint64_t>(c.outputs[i]) % size == 0),
                 "%s: misaligned pointer of tensor %d", name, i);
@@ -513,7 +562,7 @@ void launch_norm(const ListCall &c, void *workspace, void *norm, int32_t norm_dt
   int64_t used = 0;
   const bool stream = streams(total_bytes(c));
   for (const int32_t dtype : kDtypes) {
-    for_lists(c.gradients, nullptr, c.numels, c.dtypes, c.count, dtype, [&](const TensorList &list) {
+    for_lists<ReadList>(c, dtype, [&](const ReadList &list) {
       const dim3 grid(static_cast<unsigned>(std::min(list.chunks, kMaxBlocks))), block(kBlockThreads);
       with_type(dtype, [&](auto t) {
         using T = decltype(t);
@@ -530,20 +579,22 @@ void launch_norm(const ListCall &c, void *workspace, void *norm, int32_t norm_dt
 void launch_scale(const ListCall &c, double max_norm, const void *norm, int32_t norm_dtype, hipStream_t s) {
   const int f64 = norm_dtype == TBE_DTYPE_F64 ? 1 : 0;
   const uint64_t bytes = total_bytes(c);
+  const bool same = in_place(c);
   // Outputs of their own push what the norm's pass has left out of the caches, unless they are streamed (240 MB: 63 us
   // a pass, 85 with plain stores); small ones are left to whoever reads them next.
-  bool apart = false;
-  for (int32_t i = 0; i < c.count; ++i) apart = apart || (c.numels[i] && c.outputs[i] != c.gradients[i]);
-  const bool stream_in = streams(bytes), stream_out = stream_in || (apart && bytes > (uint64_t{32} << 20));
+  const bool stream_in = streams(bytes), stream_out = stream_in || (!same && bytes > (uint64_t{32} << 20));
   for (const int32_t dtype : kDtypes) {
-    for_lists(c.gradients, c.outputs, c.numels, c.dtypes, c.count, dtype, [&](const TensorList &list) {
-      const dim3 grid(static_cast<unsigned>(std::min(list.chunks, kMaxGrid))), block(kWideThreads);
-      with_type(dtype, [&](auto t) {
-        using T = decltype(t);
-        if (stream_in) TBE_LAUNCH("gradient_scale", s, (scale_kernel<T, true, true>), grid, block, list, norm, f64, max_norm);
-        else if (stream_out) TBE_LAUNCH("gradient_scale", s, (scale_kernel<T, false, true>), grid, block, list, norm, f64, max_norm);
-        else TBE_LAUNCH("gradient_scale", s, (scale_kernel<T, false, false>), grid, block, list, norm, f64, max_norm);
-      });
+    with_type(dtype, [&](auto t) {
+      using T = decltype(t);
+      const auto launch = [&](const auto &list) {
+        using L = std::decay_t<decltype(list)>;
+        const dim3 grid(static_cast<unsigned>(std::min(list.chunks, kScaleBlocks))), block(kWideThreads);
+        if (stream_in) TBE_LAUNCH("gradient_scale", s, (scale_kernel<T, L, true, true>), grid, block, list, norm, f64, max_norm);
+        else if (stream_out) TBE_LAUNCH("gradient_scale", s, (scale_kernel<T, L, false, true>), grid, block, list, norm, f64, max_norm);
+        else TBE_LAUNCH("gradient_scale", s, (scale_kernel<T, L, false, false>), grid, block, list, norm, f64, max_norm);
+      };
+      if (same) for_lists<ReadList>(c, dtype, launch);
+      else for_lists<PairList>(c, dtype, launch);
     });
   }
 }
@@ -553,20 +604,23 @@ void launch_scale(const ListCall &c, double max_norm, const void *norm, int32_t 
 bool launch_few(const ListCall &c, double max_norm, void *norm, int32_t norm_dtype, hipStream_t s) {
   int32_t dtype = -1;
   int64_t tensors = 0, chunks = 0;
+  const bool same = !c.outputs || in_place(c);
   for (int32_t i = 0; i < c.count; ++i) {
     if (c.numels[i] == 0) continue;
     if (dtype >= 0 && c.dtypes[i] != dtype) return false;
     dtype = c.dtypes[i];
     ++tensors;
-    chunks += chunks_of(c.numels[i], dtype);
-    if (tensors > kListTensors || chunks > kFewChunks) return false;
+    chunks += chunks_of(c.numels[i], reinterpret_cast<uint64_t>(same ? c.gradients[i] : c.outputs[i]), dtype).count;
+    if (tensors > kPairTensors || chunks > kFewChunks) return false;
   }
   if (tensors == 0) return false;
-  for_lists(c.gradients, c.outputs, c.numels, c.dtypes, c.count, dtype, [&](const TensorList &list) {
-    with_type(dtype, [&](auto t) {
-      TBE_LAUNCH("gradient_clip_few", s, (clip_few_kernel<decltype(t)>), dim3(1), dim3(kWideThreads), list,
-                 c.outputs ? 1 : 0, norm, norm_dtype == TBE_DTYPE_F64 ? 1 : 0, max_norm);
-    });
+  with_type(dtype, [&](auto t) {
+    const auto launch = [&](const auto &list) {
+      TBE_LAUNCH("gradient_clip_few", s, (clip_few_kernel<decltype(t), std::decay_t<decltype(list)>>), dim3(1),
+                 dim3(kWideThreads), list, c.outputs ? 1 : 0, norm, norm_dtype == TBE_DTYPE_F64 ? 1 : 0, max_norm);
+    };
+    if (same) for_lists<ReadList>(c, dtype, launch);
+    else for_lists<PairList>(c, dtype, launch);
   });
   return true;
 }
@@ -597,15 +651,16 @@ struct TableCall {
 
 template <typename T, int VEC> unsigned launch_table(const TableCall &c, int64_t tiles, int column_blocks) {
   using A = typename AccOf<T>::type;
-  const dim3 grid(static_cast<unsigned>(ceil_div(tiles, kWavesPerBlock)), column_blocks), block(kBlockThreads);
+  const int64_t per_xcd = ceil_div(ceil_div(tiles, kWavesPerBlock), kNumXcd);
+  const dim3 grid(static_cast<unsigned>(per_xcd * kNumXcd), column_blocks), block(kBlockThreads);
   const T *grad = static_cast<const T *>(c.grad), *psw = static_cast<const T *>(c.psw);
   A *rows = static_cast<A *>(c.partial_rows);
   if (psw)
     TBE_LAUNCH("table_norm_tiles", c.stream, (table_norm_tiles_kernel<T, VEC, true>), grid, block, grad, psw,
-               c.positions_sorted, c.grad_rows, c.segment_ids, c.n, c.D, tiles, rows, c.tile_sums);
+               c.positions_sorted, c.grad_rows, c.segment_ids, c.n, c.D, tiles, per_xcd, rows, c.tile_sums);
   else
     TBE_LAUNCH("table_norm_tiles", c.stream, (table_norm_tiles_kernel<T, VEC, false>), grid, block, grad, psw,
-               c.positions_sorted, c.grad_rows, c.segment_ids, c.n, c.D, tiles, rows, c.tile_sums);
+               c.positions_sorted, c.grad_rows, c.segment_ids, c.n, c.D, tiles, per_xcd, rows, c.tile_sums);
   const unsigned join = static_cast<unsigned>(std::min<int64_t>(ceil_div(tiles, kWavesPerBlock), kJoinBlocks));
   TBE_LAUNCH("table_norm_join", c.stream, (table_norm_join_kernel<T, VEC>), dim3(join), block, c.segment_ids,
              c.segment_starts, c.n, c.D, tiles, rows, c.tile_sums, column_blocks, c.partial);
