@@ -86,13 +86,6 @@ template <typename T, typename L> __device__ __forceinline__ Piece<T> piece_of_c
 
 __device__ __forceinline__ double square(double x) { return x * x; }
 
-// What the lanes of this wavefront have written to LDS is there for its other lanes.
-__device__ __forceinline__ void wave_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-}
-
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
   for (int m = 1; m < kWave; m <<= 1) v += shfl_x(v, m);
@@ -226,146 +219,127 @@ __global__ __launch_bounds__(kWideThreads) void clip_few_kernel(L list, int scal
 }
 
 // --------------------------------------------------------------------- norm of the tables' gradient
-// One wavefront per tile of kTile consecutive sorted positions and column block of up to 64 vectors; each of
-// its lane groups (one 16-byte vector of the row per lane) walks a run of consecutive positions, adding rows of
-// one segment and squaring the sum where the segment ends.  No sum over lanes is needed before the very end:
-// a lane squares its own columns.  A segment that crosses the ends of runs leaves partial sums in LDS, which lane
-// group 0 joins; one that crosses the ends of tiles leaves partial rows (row 2 * tile: what ends in the
+// One workgroup per tile of kTile consecutive sorted positions and column block of up to 64 vectors.  Its lane groups (one
+// 16-byte vector of the row per lane) each walk a run of consecutive positions, adding the gradient rows of one
+// segment and squaring the sum where the segment ends: a lane squares its own columns, so that no sum over lanes is
+// needed before the very end.  A segment that crosses runs is joined by the group in whose run it begins: what the
+// runs behind it have left of it is in LDS.  One that crosses tiles leaves partial rows (row 2 * tile: what ends in the
 // tile or runs through it, row 2 * tile + 1: what begins in it and goes on), which the next launch joins from
 // the tile where the segment begins.
+// What bounds it is the gather of the gradient rows from the caches (5.2 M lookups of 512 bytes); the workgroups of an
+// XCD walk one eighth of the positions in order, so that they work on one table's gradient rows, which its L2 holds.
 constexpr int kTile = 256;
+static_assert(kTile == kBlockThreads, "a thread per position");
 
 template <typename T, int VEC, bool WEIGHTED>
 __global__ __launch_bounds__(kBlockThreads) void table_norm_tiles_kernel(
     const T *__restrict__ grad, const T *__restrict__ psw, const int32_t *__restrict__ positions_sorted,
     const int32_t *__restrict__ grad_rows, const int32_t *__restrict__ segment_ids, int64_t n, int D,
-    int64_t num_tiles, int64_t blocks_per_xcd, typename AccOf<T>::type *__restrict__ partial_rows,
+    int64_t num_tiles, int64_t tiles_per_xcd, typename AccOf<T>::type *__restrict__ partial_rows,
     double *__restrict__ tile_sums) {
   using V = RowVec<T, VEC>;
   using A = typename V::A;
   using R = typename V::R;
   constexpr int kAhead = 8;
-  __shared__ int32_t s_segment[kWavesPerBlock][kTile];
-  __shared__ int32_t s_row[kWavesPerBlock][kTile];
-  __shared__ A s_weight[WEIGHTED ? kWavesPerBlock : 1][WEIGHTED ? kTile : 1];
-  __shared__ A s_head[kWavesPerBlock][kWave][VEC];
-  __shared__ A s_tail[kWavesPerBlock][kWave][VEC];
-  const int lane = threadIdx.x & (kWave - 1);
-  const int wave = threadIdx.x >> 6;
-  // (the workgroups of an XCD walk one eighth of the sorted positions, so that a table's gradient rows stay in its L2)
-  const int64_t tile = xcd_contiguous(blockIdx.x, blocks_per_xcd) * kWavesPerBlock + wave;
+  constexpr int kEnds = INT32_MIN;
+  __shared__ int32_t s_row[kTile];  // gradient row of every position, kEnds or'ed in where a segment ends
+  __shared__ A s_weight[WEIGHTED ? kTile : 1];
+  __shared__ A s_head[kBlockThreads][VEC];
+  __shared__ int32_t s_through[kTile];  // whether one segment runs through a whole run
+  const int64_t tile = xcd_contiguous(blockIdx.x, tiles_per_xcd);
   if (tile >= num_tiles) return;
   const int64_t p0 = tile * kTile;
   const int len = static_cast<int>(min(n - p0, static_cast<int64_t>(kTile)));
-#pragma unroll
-  for (int q = 0; q < kTile / kWave; ++q) {
-    const int i = q * kWave + lane;
-    const int64_t p = p0 + min(i, len - 1);
+  {
+    const int64_t p = min(p0 + threadIdx.x, n - 1);
     const int pos = positions_sorted[p];
-    s_segment[wave][i] = segment_ids[p];
-    s_row[wave][i] = grad_rows[pos];
-    if constexpr (WEIGHTED) s_weight[wave][i] = to_acc(psw[pos]);
+    const bool ends = p + 1 == n || segment_ids[p] != segment_ids[min(p + 1, n - 1)];
+    s_row[threadIdx.x] = grad_rows[pos] | (ends ? kEnds : 0);
+    if constexpr (WEIGHTED) s_weight[threadIdx.x] = to_acc(psw[pos]);
   }
-  wave_sync();
-  const bool open_before = p0 > 0 && segment_ids[max(p0 - 1, int64_t{0})] == s_segment[wave][0];
-  const bool open_after = p0 + len < n && segment_ids[min(p0 + len, n - 1)] == s_segment[wave][len - 1];
+  const bool open_before = p0 > 0 && segment_ids[p0 - 1] == segment_ids[p0];
+  __syncthreads();
 
-  const int vectors = D / VEC - blockIdx.y * kWave;      // of the columns from this block's first on
+  const int vectors = D / VEC - blockIdx.y * kWave;  // of the columns from this block's first on
   const int chunks = vectors < kWave ? vectors : kWave;
-  const int groups = kWave / chunks;
-  const int run = (len + groups - 1) / groups;
-  const int r = lane / chunks;
-  const int c = lane - r * chunks;
+  const int groups = kWave / chunks;                 // of a wavefront
+  const int lane = threadIdx.x & (kWave - 1);
+  const int in_wave = lane / chunks;
+  const int c = lane - in_wave * chunks;
+  const int runs = groups * kWavesPerBlock;
+  const int run = (len + runs - 1) / runs;
+  const int r = (threadIdx.x >> 6) * groups + in_wave;
   const int64_t col = (static_cast<int64_t>(blockIdx.y) * kWave + c) * VEC;
   const int begin = min(r * run, len), end = min(begin + run, len);
-  auto opens = [&](int b) { return b == 0 ? open_before : s_segment[wave][b - 1] == s_segment[wave][b]; };
-  auto goes_on = [&](int e) { return e == len ? open_after : s_segment[wave][e - 1] == s_segment[wave][e]; };
+  const bool active = in_wave < groups && begin < end;
+  // whether the position before b (behind which a run begins) belongs to the segment of position b
+  const auto opens = [&](int b) { return b == 0 ? open_before : s_row[b - 1] >= 0; };
 
   double squares = 0.0;
-  if (r < groups && begin < end) {
-    V G;
-    G.zero();
-    bool head = opens(begin);  // the segment being added began before this run
-    int current = s_segment[wave][begin];
-    auto close = [&]() {
-      if (head) {
+  V G;
+  G.zero();
+  bool head = active && opens(begin);  // the segment being added began before this run
+  const auto square = [&](const A(&g)[VEC]) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) s_head[wave][lane][k] = G.v[k];
-        head = false;
-      } else {
+    for (int k = 0; k < VEC; ++k) squares += static_cast<double>(g[k]) * static_cast<double>(g[k]);
+  };
+  const auto leave_head = [&] {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) squares += static_cast<double>(G.v[k]) * static_cast<double>(G.v[k]);
-      }
-      G.zero();
-    };
+    for (int k = 0; k < VEC; ++k) s_head[r * chunks + c][k] = G.v[k];
+  };
+  if (active) {
     for (int i0 = begin; i0 < end; i0 += kAhead) {
       R raw[kAhead];
+      int word[kAhead];
 #pragma unroll
       for (int q = 0; q < kAhead; ++q) {
-        const int i = min(i0 + q, end - 1);  // clamped, not predicated: no branch per load
-        raw[q] = V::load_raw(grad + static_cast<int64_t>(s_row[wave][i]) * D + col);
+        word[q] = s_row[min(i0 + q, end - 1)];  // clamped, not predicated: no branch per load
+        raw[q] = V::load_raw(grad + static_cast<int64_t>(word[q] & ~kEnds) * D + col);
       }
 #pragma unroll
       for (int q = 0; q < kAhead; ++q) {
-        const int i = i0 + q;
-        if (i >= end) break;
-        const int segment = s_segment[wave][i];
-        if (segment != current) {
-          close();
-          current = segment;
-        }
+        if (i0 + q >= end) break;
         V x;
         x.unpack(raw[q]);
         A w = A(1);
-        if constexpr (WEIGHTED) w = s_weight[wave][i];
+        if constexpr (WEIGHTED) w = s_weight[i0 + q];
 #pragma unroll
         for (int k = 0; k < VEC; ++k) G.v[k] += WEIGHTED ? x.v[k] * w : x.v[k];
-      }
-    }
-    if (goes_on(end) && !head) {
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) s_tail[wave][lane][k] = G.v[k];
-    } else {
-      close();  // (a segment that runs through the whole run is kept like one that ends in it)
-    }
-  }
-  wave_sync();
-  if (r == 0) {
-    V open;
-    open.zero();
-    bool from_before = open_before;
-    A *rows = partial_rows + 2 * tile * D + col;
-    for (int g = 0; g < groups; ++g) {
-      const int b = min(g * run, len), e = min(b + run, len);
-      if (b >= e) break;
-      const bool through = opens(b) && goes_on(e) && s_segment[wave][b] == s_segment[wave][e - 1];
-      if (opens(b)) {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) open.v[k] += s_head[wave][g * chunks + c][k];
-        if (through) continue;
-        if (from_before) {
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) rows[k] = open.v[k];
-          from_before = false;
-        } else {
-#pragma unroll
-          for (int k = 0; k < VEC; ++k) squares += static_cast<double>(open.v[k]) * static_cast<double>(open.v[k]);
+        if (word[q] < 0) {
+          if (head) leave_head();
+          else square(G.v);
+          head = false;
+          G.zero();
         }
-        open.zero();
-      }
-      if (goes_on(e)) {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) open.v[k] = s_tail[wave][g * chunks + c][k];
       }
     }
-    if (open_after) {
-      if (!from_before) rows += D;
+    if (head) leave_head();
+    if (c == 0) s_through[r] = head;
+  }
+  __syncthreads();
+  // The groups with a segment to join: the one in whose run it begins, and the first one for what comes from before.
+  const bool begins_here = active && !head && s_row[end - 1] >= 0;
+  for (int from = 0; from < 2; ++from) {
+    const bool joins = from == 0 ? begins_here : (active && r == 0 && open_before);
+    if (!joins) continue;
+    if (from == 1) G.zero();
+    bool open = true;
+    int t = from == 0 ? r + 1 : 0;
+    for (; open && t * run < len; ++t) {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) rows[k] = open.v[k];
+      for (int k = 0; k < VEC; ++k) G.v[k] += s_head[t * chunks + c][k];
+      open = s_through[t];
+    }
+    if (from == 0 && !open) {
+      square(G.v);
+    } else {
+      A *rows = partial_rows + (2 * tile + (from == 0 ? 1 : 0)) * D + col;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) rows[k] = G.v[k];
     }
   }
-  squares = wave_sum(squares);
-  if (lane == 0) tile_sums[tile * gridDim.y + blockIdx.y] = squares;
+  squares = block_sum<kWavesPerBlock>(squares);
+  if (threadIdx.x == 0) tile_sums[tile * gridDim.y + blockIdx.y] = squares;
 }
 
 // The segments that cross tiles: a wavefront per tile, working where one begins and goes on, adds the
@@ -374,8 +348,9 @@ template <typename T, int VEC>
 __global__ __launch_bounds__(kBlockThreads) void table_norm_join_kernel(
     const int32_t *__restrict__ segment_ids, const int32_t *__restrict__ segment_starts, int64_t n, int D,
     int64_t num_tiles, const typename AccOf<T>::type *__restrict__ partial_rows,
-    const double *__restrict__ tile_sums, int column_blocks, double *__restrict__ partial) {
+    const double *__restrict__ tile_sums, int column_blocks, double *__restrict__ partial, void *norm, int f64) {
   using A = typename AccOf<T>::type;
+  constexpr int kAhead = 8;
   const int lane = threadIdx.x & (kWave - 1);
   double squares = 0.0;  // (of this lane)
   const int64_t stride = static_cast<int64_t>(gridDim.x) * kWavesPerBlock;
@@ -398,10 +373,22 @@ __global__ __launch_bounds__(kBlockThreads) void table_norm_join_kernel(
 #pragma unroll
       for (int k = 0; k < VEC; ++k) sum[k] = A(0);
       if (r < groups) {
-        for (int64_t t = tile + r; t <= last; t += groups) {
-          const A *row = partial_rows + (2 * t + (t == tile ? 1 : 0)) * D + col;
+        // (eight partial rows are requested before the first is added)
+        for (int64_t t0 = tile + r; t0 <= last; t0 += groups * kAhead) {
+          A part[kAhead][VEC];
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) sum[k] += row[k];
+          for (int a = 0; a < kAhead; ++a) {
+            const int64_t t = min(t0 + a * groups, last);
+            const A *row = partial_rows + (2 * t + (t == tile ? 1 : 0)) * D + col;
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) part[a][k] = row[k];
+          }
+#pragma unroll
+          for (int a = 0; a < kAhead; ++a) {
+            const bool real = t0 + a * groups <= last;
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) sum[k] += real ? part[a][k] : A(0);
+          }
         }
       }
       for (int g = 1; g < groups; ++g) {
@@ -419,13 +406,16 @@ __global__ __launch_bounds__(kBlockThreads) void table_norm_join_kernel(
     }
   }
   squares = block_sum<kWavesPerBlock>(squares);
-  if (threadIdx.x == 0) partial[blockIdx.x] = squares;
+  if (threadIdx.x != 0) return;
+  if (gridDim.x == 1) store_norm(norm, f64, squares);  // (no more launches: this is all of it)
+  else partial[blockIdx.x] = squares;
 }
 
 // ------------------------------------------------------------------------------------------ host
 constexpr int kMaxBlocks = 256 * 8;   // of a sum over a list: eight workgroups per compute unit
 constexpr int kScaleBlocks = 1 << 14; // of a scaling launch (see scale_kernel)
-constexpr int kJoinBlocks = 1024;
+constexpr int kJoinBlocks = 8192;
+constexpr int kFewTiles = 8;
 
 size_t size_of(int32_t dtype) { return dtype == TBE_DTYPE_F64 ? 8 : dtype == TBE_DTYPE_F32 ? 4 : 2; }
 
@@ -646,12 +636,15 @@ struct TableCall {
   int32_t D;
   void *partial_rows;
   double *tile_sums, *partial;
+  void *norm;
+  int f64;
   hipStream_t stream;
 };
 
+// Returns the number of partial sums left, 0 if the norm is written.
 template <typename T, int VEC> unsigned launch_table(const TableCall &c, int64_t tiles, int column_blocks) {
   using A = typename AccOf<T>::type;
-  const int64_t per_xcd = ceil_div(ceil_div(tiles, kWavesPerBlock), kNumXcd);
+  const int64_t per_xcd = ceil_div(tiles, kNumXcd);
   const dim3 grid(static_cast<unsigned>(per_xcd * kNumXcd), column_blocks), block(kBlockThreads);
   const T *grad = static_cast<const T *>(c.grad), *psw = static_cast<const T *>(c.psw);
   A *rows = static_cast<A *>(c.partial_rows);
@@ -661,10 +654,11 @@ template <typename T, int VEC> unsigned launch_table(const TableCall &c, int64_t
   else
     TBE_LAUNCH("table_norm_tiles", c.stream, (table_norm_tiles_kernel<T, VEC, false>), grid, block, grad, psw,
                c.positions_sorted, c.grad_rows, c.segment_ids, c.n, c.D, tiles, per_xcd, rows, c.tile_sums);
-  const unsigned join = static_cast<unsigned>(std::min<int64_t>(ceil_div(tiles, kWavesPerBlock), kJoinBlocks));
+  // a tile per wavefront, or one workgroup for what that can do in the time of a launch
+  const unsigned join = tiles <= kFewTiles ? 1 : static_cast<unsigned>(std::min<int64_t>(ceil_div(tiles, kWavesPerBlock), kJoinBlocks));
   TBE_LAUNCH("table_norm_join", c.stream, (table_norm_join_kernel<T, VEC>), dim3(join), block, c.segment_ids,
-             c.segment_starts, c.n, c.D, tiles, rows, c.tile_sums, column_blocks, c.partial);
-  return join;
+             c.segment_starts, c.n, c.D, tiles, rows, c.tile_sums, column_blocks, c.partial, c.norm, c.f64);
+  return join == 1 ? 0 : join;
 }
 
 }  // namespace
@@ -751,7 +745,8 @@ extern "C" int tbe_table_gradient_norm(const void *grad_output, int32_t dtype, i
   // The update's queues and partial rows are not in use between a plan and its update: the tiles' sums go to the
   // chunk records' room, the partial rows (two per kTile positions, like the update's) to their own.
   static_assert(kTile == kChunkLen, "two partial rows per tile fit the update's");
-  const uint64_t sums = static_cast<uint64_t>(tiles * column_blocks + kJoinBlocks) * sizeof(double);
+  const int64_t join_parts = std::min<int64_t>(ceil_div(tiles, kWavesPerBlock), kJoinBlocks);
+  const uint64_t sums = static_cast<uint64_t>(tiles * column_blocks + join_parts) * sizeof(double);
   if (sums > l.partial_sums - l.chunk_segments || column_blocks > 65535)
     return fail(TBE_ERR_UNSUPPORTED, "%s: rows of %d elements are too wide", name, D);
   char *ws = static_cast<char *>(workspace);
@@ -766,7 +761,9 @@ extern "C" int tbe_table_gradient_norm(const void *grad_output, int32_t dtype, i
   c.D = D;
   c.partial_rows = ws + l.partial_sums;
   c.partial = reinterpret_cast<double *>(ws + l.chunk_segments);
-  c.tile_sums = c.partial + kJoinBlocks;
+  c.tile_sums = c.partial + join_parts;
+  c.norm = norm;
+  c.f64 = f64;
   c.stream = s;
   unsigned parts;
   switch (dtype) {
@@ -777,7 +774,8 @@ extern "C" int tbe_table_gradient_norm(const void *grad_output, int32_t dtype, i
       break;
     default: parts = launch_table<double, 2>(c, tiles, static_cast<int>(column_blocks)); break;
   }
-  TBE_LAUNCH("gradient_norm", s, norm_finish_kernel, dim3(1), dim3(kWideThreads), c.partial,
-             static_cast<int64_t>(parts), norm, f64);
+  if (parts)
+    TBE_LAUNCH("gradient_norm", s, norm_finish_kernel, dim3(1), dim3(kWideThreads), c.partial,
+               static_cast<int64_t>(parts), norm, f64);
   return check_launch(name);
 }
