@@ -103,23 +103,22 @@ template <int WAVES> __device__ __forceinline__ double block_sum(double v) {
   return sum;
 }
 
-// This thread's squares of a chunk that THREADS threads share.
-template <typename T, int THREADS, bool STREAM>
+// This thread's squares of a chunk that THREADS threads share; AHEAD vectors are requested before the first is used.
+template <typename T, int THREADS, int AHEAD, bool STREAM>
 __device__ __forceinline__ double chunk_squares(const Piece<T> &p, int thread) {
   constexpr int kVec = 16 / sizeof(T);
-  constexpr int kAhead = 4;
   const T *src = p.src;
   const int vectors = p.count / kVec;
   double sum = 0.0;
-  for (int i0 = thread; i0 < vectors; i0 += THREADS * kAhead) {
-    Pack<T, kVec> x[kAhead];
+  for (int i0 = thread; i0 < vectors; i0 += THREADS * AHEAD) {
+    Pack<T, kVec> x[AHEAD];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
+    for (int u = 0; u < AHEAD; ++u) {
       const int i = i0 + u * THREADS;
       x[u] = load_pack<T, kVec, STREAM>(src + min(i, vectors - 1) * kVec);  // clamped: no branch per load
     }
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
+    for (int u = 0; u < AHEAD; ++u) {
       if (i0 + u * THREADS >= vectors) break;
 #pragma unroll
       for (int q = 0; q < kVec; ++q) sum += square(static_cast<double>(x[u].v[q]));
@@ -133,18 +132,26 @@ __device__ __forceinline__ double chunk_squares(const Piece<T> &p, int thread) {
 
 // dst = src * scale for a chunk that THREADS threads share: products in 32 bits for the types of up to 32, rounded
 // once more for those of 16.
-template <typename T, int THREADS, bool STREAM_IN, bool STREAM_OUT>
+template <typename T, int THREADS, int AHEAD, bool STREAM_IN, bool STREAM_OUT>
 __device__ __forceinline__ void chunk_scaled(const Piece<T> &p, typename AccOf<T>::type scale, int thread) {
   using A = typename AccOf<T>::type;
   constexpr int kVec = 16 / sizeof(T);
   const T *src = p.src;
   T *dst = p.dst;
   const int vectors = p.count / kVec;
-  for (int i = thread; i < vectors; i += THREADS) {
-    Pack<T, kVec> x = load_pack<T, kVec, STREAM_IN>(src + i * kVec);
+  for (int i0 = thread; i0 < vectors; i0 += THREADS * AHEAD) {
+    Pack<T, kVec> x[AHEAD];
 #pragma unroll
-    for (int q = 0; q < kVec; ++q) x.v[q] = static_cast<T>(static_cast<A>(x.v[q]) * scale);
-    store_pack<T, kVec, STREAM_OUT>(dst + i * kVec, x);
+    for (int u = 0; u < AHEAD; ++u)
+      x[u] = load_pack<T, kVec, STREAM_IN>(src + min(i0 + u * THREADS, vectors - 1) * kVec);
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int i = i0 + u * THREADS;
+      if (i >= vectors) break;
+#pragma unroll
+      for (int q = 0; q < kVec; ++q) x[u].v[q] = static_cast<T>(static_cast<A>(x[u].v[q]) * scale);
+      store_pack<T, kVec, STREAM_OUT>(dst + i * kVec, x[u]);
+    }
   }
   const int rest = vectors * kVec + thread;
   if (rest < p.count) dst[rest] = static_cast<T>(static_cast<A>(src[rest]) * scale);
@@ -168,7 +175,7 @@ template <typename T, bool STREAM>
 __global__ __launch_bounds__(kBlockThreads) void square_sum_kernel(ReadList list, double *__restrict__ partial) {
   double sum = 0.0;
   for (int chunk = blockIdx.x; chunk < list.chunks; chunk += gridDim.x)
-    sum += chunk_squares<T, kBlockThreads, STREAM>(piece_of_chunk<T>(list, chunk), threadIdx.x);
+    sum += chunk_squares<T, kBlockThreads, 4, STREAM>(piece_of_chunk<T>(list, chunk), threadIdx.x);
   sum = block_sum<kWavesPerBlock>(sum);
   if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
@@ -193,7 +200,7 @@ __global__ __launch_bounds__(kWideThreads) void scale_kernel(L list, const void 
   const A scale = static_cast<A>(clip_scale(n, max_norm));
   if (!L::kPairs && scale == A(1)) return;  // in place and within the limit: nothing changes
   for (int chunk = blockIdx.x; chunk < list.chunks; chunk += gridDim.x)
-    chunk_scaled<T, kWideThreads, STREAM_IN, STREAM_OUT>(piece_of_chunk<T>(list, chunk), scale, threadIdx.x);
+    chunk_scaled<T, kWideThreads, 1, STREAM_IN, STREAM_OUT>(piece_of_chunk<T>(list, chunk), scale, threadIdx.x);
 }
 
 // Few chunks: norm and scaling in one workgroup, a wavefront per chunk.
@@ -207,7 +214,7 @@ __global__ __launch_bounds__(kWideThreads) void clip_few_kernel(L list, int scal
   const int wave = threadIdx.x >> 6;
   double sum = 0.0;
   for (int chunk = wave; chunk < list.chunks; chunk += kWaves)
-    sum += chunk_squares<T, kWave, false>(piece_of_chunk<T>(list, chunk), lane);
+    sum += chunk_squares<T, kWave, 8, false>(piece_of_chunk<T>(list, chunk), lane);
   sum = block_sum<kWaves>(sum);
   if (threadIdx.x == 0) store_norm(norm, f64, sum);
   if (!scaled) return;
@@ -215,7 +222,7 @@ __global__ __launch_bounds__(kWideThreads) void clip_few_kernel(L list, int scal
   const A scale = static_cast<A>(clip_scale(n, max_norm));
   if (!L::kPairs && scale == A(1)) return;
   for (int chunk = wave; chunk < list.chunks; chunk += kWaves)
-    chunk_scaled<T, kWave, false, false>(piece_of_chunk<T>(list, chunk), scale, lane);
+    chunk_scaled<T, kWave, 8, false, false>(piece_of_chunk<T>(list, chunk), scale, lane);
 }
 
 // --------------------------------------------------------------------- norm of the tables' gradient
