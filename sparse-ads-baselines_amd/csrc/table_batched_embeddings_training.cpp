@@ -18,6 +18,8 @@
 namespace tbe_binding {
 namespace {
 
+namespace py = pybind11;
+
 // element types of expert routing and clipping: those of the tables and bfloat16
 int32_t float_code(const at::Tensor &t, const char *name) {
   switch (t.scalar_type()) {
@@ -202,6 +204,25 @@ at::Tensor expert_combine(const at::Tensor &rows, const at::Tensor &places, cons
 }
 
 // -------------------------------------------------------------------- gradient norm and clipping
+// The tensors of a Python sequence (or any iterable), looked at where they are: lists of hundreds of tensors are bound
+// by what the host does for each of them.
+class TensorSequence {
+ public:
+  TensorSequence(const py::object &source, const char *name)
+      : items_(py::reinterpret_steal<py::object>(PySequence_Fast(source.ptr(), "a list of tensors is needed"))) {
+    if (!items_) throw py::error_already_set();
+    const Py_ssize_t count = size();
+    for (Py_ssize_t i = 0; i < count; ++i)
+      TORCH_CHECK_TYPE(THPVariable_Check(item(i)), name, " must be tensors (entry ", i, " is none)");
+  }
+  Py_ssize_t size() const { return PySequence_Fast_GET_SIZE(items_.ptr()); }
+  const at::Tensor &operator[](Py_ssize_t i) const { return THPVariable_Unpack(item(i)); }
+
+ private:
+  PyObject *item(Py_ssize_t i) const { return PySequence_Fast_GET_ITEM(items_.ptr(), i); }
+  py::object items_;
+};
+
 struct GradientList {
   std::vector<const void *> gradients;
   std::vector<void *> outputs;
@@ -211,17 +232,18 @@ struct GradientList {
   int32_t count() const { return static_cast<int32_t>(gradients.size()); }
 };
 
-GradientList check_gradients(const std::vector<at::Tensor> &gradients, const std::vector<at::Tensor> *outputs) {
-  TORCH_CHECK(!gradients.empty(), "there must be at least one gradient");
-  TORCH_CHECK(gradients.size() < (1u << 24), "too many gradients");
-  TORCH_CHECK(!outputs || outputs->size() == gradients.size(), "out must hold one tensor per gradient");
+GradientList check_gradients(const TensorSequence &gradients, const TensorSequence *outputs) {
+  const Py_ssize_t count = gradients.size();
+  TORCH_CHECK(count > 0, "there must be at least one gradient");
+  TORCH_CHECK(count < (1 << 24), "too many gradients");
+  TORCH_CHECK(!outputs || outputs->size() == count, "out must hold one tensor per gradient");
   GradientList list;
-  list.gradients.reserve(gradients.size());
-  list.numels.reserve(gradients.size());
-  list.dtypes.reserve(gradients.size());
-  list.outputs.reserve(gradients.size());
+  list.gradients.reserve(count);
+  list.numels.reserve(count);
+  list.dtypes.reserve(count);
+  list.outputs.reserve(count);
   const at::Device device = gradients[0].device();
-  for (size_t i = 0; i < gradients.size(); ++i) {
+  for (Py_ssize_t i = 0; i < count; ++i) {
     const at::Tensor &g = gradients[i];
     TORCH_CHECK(g.is_cuda(), "gradients must be GPU tensors");
     TORCH_CHECK(g.layout() == at::kStrided, "gradients must be strided (dense) tensors");
@@ -232,11 +254,14 @@ GradientList check_gradients(const std::vector<at::Tensor> &gradients, const std
     list.f64 = list.f64 || g.scalar_type() == at::kDouble;
     list.gradients.push_back(g.data_ptr());
     list.numels.push_back(g.numel());
-    const at::Tensor &o = outputs ? (*outputs)[i] : g;
-    if (outputs)
-      TORCH_CHECK(o.device() == device && o.scalar_type() == g.scalar_type() && o.sizes() == g.sizes() &&
-                      o.strides() == g.strides(),
-                  "out must have the gradients' shapes, strides, types and device (tensor ", i, ")");
+    if (!outputs) {
+      list.outputs.push_back(g.data_ptr());
+      continue;
+    }
+    const at::Tensor &o = (*outputs)[i];
+    TORCH_CHECK(o.device() == device && o.layout() == at::kStrided && o.scalar_type() == g.scalar_type() &&
+                    o.sizes() == g.sizes() && o.strides() == g.strides(),
+                "out must have the gradients' shapes, strides, types and device (tensor ", i, ")");
     list.outputs.push_back(o.data_ptr());
   }
   return list;
@@ -247,31 +272,37 @@ at::Tensor empty_norm(const at::Tensor &like, bool f64) {
 }
 int32_t norm_code(bool f64) { return f64 ? TBE_DTYPE_F64 : TBE_DTYPE_F32; }
 
-at::Tensor gradient_norm(const std::vector<at::Tensor> &gradients) {
+at::Tensor gradient_norm(const py::object &source) {
+  const TensorSequence gradients(source, "gradients");
   const GradientList list = check_gradients(gradients, nullptr);
-  c10::DeviceGuard guard(gradients[0].device());
-  at::Tensor norm = empty_norm(gradients[0], list.f64);
+  const at::Tensor &first = gradients[0];
+  c10::DeviceGuard guard(first.device());
+  at::Tensor norm = empty_norm(first, list.f64);
   const uint64_t bytes = tbe_gradient_norm_workspace_bytes(list.count());
-  at::Tensor scratch = at::empty({static_cast<int64_t>(bytes)}, gradients[0].options().dtype(at::kByte));
+  at::Tensor scratch = at::empty({static_cast<int64_t>(bytes)}, first.options().dtype(at::kByte));
   check(tbe_gradient_norm(list.gradients.data(), list.numels.data(), list.dtypes.data(), list.count(), norm.data_ptr(),
-                          norm_code(list.f64), scratch.data_ptr(), bytes, stream_of(gradients[0])));
+                          norm_code(list.f64), scratch.data_ptr(), bytes, stream_of(first)));
   return norm;
 }
 
-at::Tensor clip_gradients(const std::vector<at::Tensor> &gradients, double max_norm,
-                          const c10::optional<std::vector<at::Tensor>> &out) {
-  const GradientList list = check_gradients(gradients, out.has_value() ? &*out : nullptr);
+at::Tensor clip_gradients(const py::object &source, double max_norm, const py::object &out) {
+  const TensorSequence gradients(source, "gradients");
+  c10::optional<TensorSequence> outputs;
+  if (!out.is_none()) outputs.emplace(out, "out");
+  const GradientList list = check_gradients(gradients, outputs.has_value() ? &*outputs : nullptr);
   TORCH_CHECK(max_norm >= 0.0, "max_norm must not be negative");
-  c10::DeviceGuard guard(gradients[0].device());
-  at::Tensor norm = empty_norm(gradients[0], list.f64);
+  const at::Tensor &first = gradients[0];
+  c10::DeviceGuard guard(first.device());
+  at::Tensor norm = empty_norm(first, list.f64);
   const uint64_t bytes = tbe_gradient_norm_workspace_bytes(list.count());
-  at::Tensor scratch = at::empty({static_cast<int64_t>(bytes)}, gradients[0].options().dtype(at::kByte));
+  at::Tensor scratch = at::empty({static_cast<int64_t>(bytes)}, first.options().dtype(at::kByte));
   check(tbe_clip_gradients(list.gradients.data(), list.outputs.data(), list.numels.data(), list.dtypes.data(),
                            list.count(), max_norm, norm.data_ptr(), norm_code(list.f64), scratch.data_ptr(), bytes,
-                           stream_of(gradients[0])));
+                           stream_of(first)));
   // autograd learns that the tensors were written
-  for (const at::Tensor &t : out.has_value() ? *out : gradients)
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  const TensorSequence &written = outputs.has_value() ? *outputs : gradients;
+  for (Py_ssize_t i = 0; i < written.size(); ++i)
+    if (!written[i].is_inference()) written[i].unsafeGetTensorImpl()->bump_version();
   return norm;
 }
 
@@ -357,7 +388,6 @@ at::Tensor backward_clipped(int64_t optimizer, at::Tensor grad_output, at::Tenso
 }  // namespace
 
 void bind_training(pybind11::module &m) {
-  namespace py = pybind11;
   using release = py::call_guard<py::gil_scoped_release>;
   m.def("expert_plan", &expert_plan, "stable order of the (token, choice) pairs by expert", py::arg("expert_ids"),
         py::arg("num_experts"), release());
@@ -368,9 +398,9 @@ void bind_training(pybind11::module &m) {
   m.def("expert_combine_backward", &combine_backward, "gradients of expert_combine", py::arg("grad_output"),
         py::arg("rows"), py::arg("places"), py::arg("expert_offsets"), py::arg("weights"), py::arg("want_rows") = true,
         py::arg("want_weights") = true, release());
-  m.def("gradient_norm", &gradient_norm, "global norm of a list of gradients", py::arg("gradients"), release());
+  m.def("gradient_norm", &gradient_norm, "global norm of a list of gradients", py::arg("gradients"));
   m.def("clip_gradients", &clip_gradients, "scales a list of gradients down to a global norm", py::arg("gradients"),
-        py::arg("max_norm"), py::arg("out") = py::none(), release());
+        py::arg("max_norm"), py::arg("out") = py::none());
   m.def("clip_table_gradient", &clip_table_gradient, "grad_output scaled by the norm of the tables' exact gradient",
         py::arg("grad_output"), py::arg("weights"), py::arg("table_offsets"), py::arg("indices"), py::arg("offsets"),
         py::arg("max_norm"), py::arg("indice_weights") = py::none(), release());

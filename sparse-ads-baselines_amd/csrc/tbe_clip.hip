@@ -504,26 +504,32 @@ int check_list(const char *name, const ListCall &c, bool outputs) {
 int check_overlap(const char *name, const ListCall &c) {
   struct Range {
     uint64_t begin, end;
-    int32_t tensor;
-    bool written;
+    bool operator<(const Range &o) const { return begin < o.begin; }
   };
   try {
-    std::vector<Range> ranges;
-    ranges.reserve(2 * static_cast<size_t>(c.count));
+    std::vector<Range> written, read;  // (a gradient that is its own output counts as written only)
+    written.reserve(c.count);
     for (int32_t i = 0; i < c.count; ++i) {
       if (c.numels[i] == 0) continue;
       const uint64_t bytes = static_cast<uint64_t>(c.numels[i]) * size_of(c.dtypes[i]);
       const uint64_t out = reinterpret_cast<uint64_t>(c.outputs[i]), in = reinterpret_cast<uint64_t>(c.gradients[i]);
-      ranges.push_back(Range{out, out + bytes, i, true});
-      if (in != out) ranges.push_back(Range{in, in + bytes, i, false});
+      written.push_back(Range{out, out + bytes});
+      if (in != out) read.push_back(Range{in, in + bytes});
     }
-    std::sort(ranges.begin(), ranges.end(), [](const Range &a, const Range &b) { return a.begin < b.begin; });
-    // the furthest ends so far, of what is written and of what is only read
-    uint64_t written_end = 0, read_end = 0;
-    for (const Range &r : ranges) {
-      TBE_REQUIRE(r.begin >= written_end && (!r.written || r.begin >= read_end),
-                  "%s: tensor %d shares memory with another one of the list", name, r.tensor);
-      (r.written ? written_end : read_end) = std::max(r.written ? written_end : read_end, r.end);
+    // (the tensors of a bucket come in order: nothing to sort then)
+    for (std::vector<Range> *v : {&written, &read})
+      if (!std::is_sorted(v->begin(), v->end())) std::sort(v->begin(), v->end());
+    size_t r = 0;
+    uint64_t read_end = 0;  // of the ranges read that begin before the one written
+    for (size_t w = 0; w < written.size(); ++w) {
+      for (; r < read.size() && read[r].begin < written[w].end; ++r) {
+        // it begins before this range's end: it has to end before its begin, and, beginning behind the ranges written
+        // before, to begin behind their ends
+        TBE_REQUIRE(w == 0 || read[r].begin >= written[w - 1].end, "%s: an output shares memory with another tensor's gradient", name);
+        read_end = std::max(read_end, read[r].end);
+      }
+      TBE_REQUIRE(read_end <= written[w].begin, "%s: an output shares memory with another tensor's gradient", name);
+      TBE_REQUIRE(w == 0 || written[w].begin >= written[w - 1].end, "%s: two outputs share memory", name);
     }
   } catch (const std::bad_alloc &) {
     return fail(TBE_ERR_INVALID, "%s: out of host memory", name);

@@ -53,7 +53,7 @@ __global__ __launch_bounds__(tile_waves(BINS) * kWave) void expert_count_kernel(
   const int64_t base = static_cast<int64_t>(blockIdx.x) * tile_pairs(BINS, ITEMS) + threadIdx.x;
   I id[ITEMS];
 #pragma unroll
-  for (int q = 0; q < ITEMS; ++q) id[q] = ids[min(base + q * kThreads, n - 1)];
+  for (int q = 0; q < ITEMS; ++q) id[q] = base + q * kThreads < n ? ids[base + q * kThreads] : I(0);
   for (int e = threadIdx.x; e <= E; e += kThreads) s_count[e] = 0;
   __syncthreads();
 #pragma unroll

@@ -67,9 +67,6 @@ class LookupFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, weights, table_offsets, indices, offsets, per_sample_weights, optimizer,
                 optimizer_state, learning_rate, eps, stochastic_rounding, clip=None):
-        if clip is not None and ctx.needs_input_grad[4]:
-            # (their gradient is formed inside the table update, from the gradient that was clipped for the tables)
-            raise RuntimeError("clip_gradient does not go with per-sample weights that need a gradient")
         ctx.clip = clip
         ctx.optimizer = optimizer
         ctx.learning_rate = learning_rate
@@ -314,6 +311,10 @@ class TableBatchedEmbeddingBags(_CacheFronted, nn.Module):
         if self.row_cache is not None:
             return CachedLookupFunction.apply(self.embedding_weights, self, sharded_sparse_features,
                                               sharded_offsets, per_sample_weights)
+        if (self.gradient_clip is not None and per_sample_weights is not None and per_sample_weights.requires_grad
+                and torch.is_grad_enabled()):
+            # (their gradient is formed inside the table update, from the gradient that was clipped for the tables)
+            raise RuntimeError("clip_gradient does not go with per-sample weights that need a gradient")
         return LookupFunction.apply(
             self.embedding_weights, self.table_offsets, sharded_sparse_features, sharded_offsets,
             per_sample_weights, self.optimizer, self.optimizer_state, self.learning_rate, self.eps,

@@ -67,10 +67,10 @@ def test_clip_refusals():
 def test_shared_memory_is_refused(addresses, outputs):
     _, scale, clip = _all(addresses, [8] * len(addresses), [0] * len(addresses), outputs, nbytes=0)
     assert scale == 1
-    assert "shares memory" in tbe_native.load().tbe_last_error().decode() or clip == 2
+    assert "share" in tbe_native.load().tbe_last_error().decode() or clip == 2
     _, scale, clip = _all(addresses, [8] * len(addresses), [0] * len(addresses), outputs)
     assert scale == clip == 1
-    assert "shares memory" in tbe_native.load().tbe_last_error().decode()
+    assert "share" in tbe_native.load().tbe_last_error().decode()
 
 
 def test_table_norm_refusals():

@@ -57,7 +57,7 @@ def make_list(seed, sizes, dtype, misalign=0, scale=0.1):
 
 
 SIZES = [[1], [7], [8, 0, 9], [1023, 1, 4096, 16385], [100003, 3, 64 * 1024 + 5], [17 + i % 300 for i in range(300)],
-         [3000001]]
+         [3000001], [1 + i % 5 for i in range(700)]]
 
 
 @pytest.mark.parametrize("sizes", SIZES, ids=lambda s: "%dx%d" % (len(s), s[0]))
@@ -178,15 +178,18 @@ def test_refusals():
             (lambda: ops.gradient_norm([g[0].expand(4, 8)]), "gaps"),
             (lambda: ops.gradient_norm([g, torch.zeros(3)]), "GPU tensors"),
             (lambda: ops.gradient_norm([g.int()]), "float16"),
-            (lambda: ops.clip_gradients([g, g], 1.0), "shares memory"),
-            (lambda: ops.clip_gradients([g, g[2]], 1.0), "shares memory"),
+            (lambda: ops.gradient_norm([g, 3.0]), "must be tensors"),
+            (lambda: ops.gradient_norm(7), "a list of tensors"),
+            (lambda: ops.clip_gradients([g, g], 1.0), "share memory"),
+            (lambda: ops.clip_gradients([g, g[2]], 1.0), "share memory"),
             (lambda: ops.clip_gradients([g], -1.0), "max_norm"),
             (lambda: ops.clip_gradients([g], float("nan")), "max_norm"),
             (lambda: ops.clip_gradients([g], 1.0, out=[]), "one tensor per"),
             (lambda: ops.clip_gradients([g], 1.0, out=[g.t()]), "strides"),
             (lambda: ops.clip_gradients([g], 1.0, out=[g.half()]), "types")]:
-        with pytest.raises(RuntimeError, match=needle):
+        with pytest.raises((RuntimeError, TypeError), match=needle):
             call()
+    assert float(ops.gradient_norm(t for t in (g, g))) == 0.0  # an iterator will do
 
 
 def test_autograd_learns_that_a_gradient_was_scaled():
@@ -360,6 +363,8 @@ def test_module_clip_refusals():
     idx, off = torch.zeros(4, dtype=torch.int32, device=DEV), torch.arange(0, 5, dtype=torch.int32, device=DEV)
     psw = torch.ones(4, device=DEV, requires_grad=True)
     with pytest.raises(RuntimeError, match="per-sample weights"):
+        m(idx, off, psw)
+    with torch.no_grad():  # no backward to come
         m(idx, off, psw)
     with pytest.raises(RuntimeError, match="max_norm"):
         m.clip_gradient(-2.0)

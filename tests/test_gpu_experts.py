@@ -91,6 +91,9 @@ def test_plan_of_transposed_and_empty_ids():
     rows = routing.dispatch(torch.empty(0, 16, device=DEV))
     assert rows.shape == (0, 16)
     assert routing.combine(rows, torch.empty(0, 4, device=DEV)).shape == (0, 16)
+    for experts in (1, 255, 1023, 1024, 4095):  # no token chose any of them
+        none = ops.ExpertRouting(torch.empty(0, 2, dtype=torch.int64, device=DEV), experts)
+        assert none.expert_offsets.numel() == experts + 1 and not none.expert_offsets.any()
 
 
 # widths around the vector widths of every type, one vector more than a workgroup's, and strides
@@ -217,6 +220,42 @@ def test_the_same_expert_twice_and_shared_weights():
     torch.testing.assert_close(y, 4 * w * x, rtol=1e-14, atol=1e-14)
     torch.testing.assert_close(gx, 4 * w * g, rtol=1e-14, atol=1e-14)
     torch.testing.assert_close(gw, 4 * (x * g).sum(1, keepdim=True), rtol=1e-13, atol=1e-13)
+
+
+def test_only_the_gradients_that_are_wanted():
+    """Frozen gates leave the rows unread, frozen rows get nothing written; the other gradient is the same."""
+    p = _problem(12, 40, 3, 6, 72, BF16, 0.2)
+    rows, weights = p["rows"].detach(), p["weights"].detach()
+    both = [rows.clone().requires_grad_(True), weights.clone().requires_grad_(True)]
+    want = torch.autograd.grad(p["routing"].combine(*both), both, p["grad"])
+    (g,) = torch.autograd.grad(p["routing"].combine(both[0], weights), both[0], p["grad"])
+    assert torch.equal(g, want[0])
+    (g,) = torch.autograd.grad(p["routing"].combine(rows, both[1]), both[1], p["grad"])
+    assert torch.equal(g, want[1])
+    assert not p["routing"].combine(rows, weights).requires_grad
+    with torch.no_grad():
+        assert not p["routing"].combine(*both).requires_grad and not p["routing"].dispatch(p["x"]).requires_grad
+
+
+def test_second_derivatives_are_refused():
+    p = _problem(13, 10, 2, 4, 16, F32, 0.0)
+    x = p["x"].detach().requires_grad_(True)
+    rows = p["routing"].dispatch(x)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(rows, x, torch.ones_like(rows), create_graph=True)
+    weights = p["weights"].requires_grad_(True)
+    y = p["routing"].combine(rows.detach(), weights)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(y, weights, torch.ones_like(y), create_graph=True)
+
+
+def test_rows_written_after_they_were_combined():
+    p = _problem(14, 10, 2, 4, 16, F32, 0.0)
+    rows, weights = p["rows"].clone(), p["weights"].requires_grad_(True)
+    y = p["routing"].combine(rows, weights)
+    rows.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
 
 
 def test_gradients_against_differences():
