@@ -349,27 +349,62 @@ __global__ __launch_bounds__(kBlockThreads) void table_norm_tiles_kernel(
   if (threadIdx.x == 0) tile_sums[tile * gridDim.y + blockIdx.y] = squares;
 }
 
+// The partial rows first, first + step, ... up to `last` of the segment that begins in `tile`, for this lane's columns;
+// eight are requested before the first is added.
+template <int VEC, typename A>
+__device__ __forceinline__ void add_partial_rows(const A *__restrict__ partial_rows, int D, int64_t tile, int64_t first,
+                                                 int64_t step, int64_t last, int64_t col, A (&sum)[VEC]) {
+  constexpr int kAhead = 8;
+  for (int64_t t0 = first; t0 <= last; t0 += step * kAhead) {
+    A part[kAhead][VEC];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const int64_t t = min(t0 + a * step, last);
+      const A *row = partial_rows + (2 * t + (t == tile ? 1 : 0)) * D + col;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) part[a][k] = row[k];
+    }
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const bool real = t0 + a * step <= last;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) sum[k] += real ? part[a][k] : A(0);
+    }
+  }
+}
+
 // The segments that cross tiles: a wavefront per tile, working where one begins and goes on, adds the
-// partial rows of the tiles up to its end; a workgroup's wavefronts then add up their tiles' squares.
+// partial rows of the tiles up to its end; a workgroup's wavefronts then add up their tiles' squares.  Segments of more
+// than kLongTiles tiles are left to the workgroups behind `joins`, one for every kLongTiles tiles: it joins the
+// segment whose first such tile is its own.  (One row looked up 5.2 million times: 201 us, 741 with a wavefront.)
+constexpr int kLongTiles = 64;
 template <typename T, int VEC>
 __global__ __launch_bounds__(kBlockThreads) void table_norm_join_kernel(
     const int32_t *__restrict__ segment_ids, const int32_t *__restrict__ segment_starts, int64_t n, int D,
-    int64_t num_tiles, const typename AccOf<T>::type *__restrict__ partial_rows,
+    int64_t num_tiles, int joins, const typename AccOf<T>::type *__restrict__ partial_rows,
     const double *__restrict__ tile_sums, int column_blocks, double *__restrict__ partial, void *norm, int f64) {
   using A = typename AccOf<T>::type;
-  constexpr int kAhead = 8;
+  __shared__ A s_part[kWavesPerBlock][kWave][VEC];
   const int lane = threadIdx.x & (kWave - 1);
+  const int wave = threadIdx.x >> 6;
+  const bool is_long = static_cast<int>(blockIdx.x) >= joins;
   double squares = 0.0;  // (of this lane)
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * kWavesPerBlock;
-  for (int64_t tile = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + (threadIdx.x >> 6); tile < num_tiles;
-       tile += stride) {
-    for (int b = lane; b < column_blocks; b += kWave) squares += tile_sums[tile * column_blocks + b];
-    const int64_t next = (tile + 1) * kTile;
+  const int64_t first = is_long ? (static_cast<int64_t>(blockIdx.x) - joins) * kLongTiles
+                                : static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + wave;
+  const int64_t stride = is_long ? num_tiles : static_cast<int64_t>(joins) * kWavesPerBlock;
+  for (int64_t at = first; at < num_tiles; at += stride) {
+    if (!is_long)
+      for (int b = lane; b < column_blocks; b += kWave) squares += tile_sums[at * column_blocks + b];
+    const int64_t next = (at + 1) * kTile;
     if (next >= n) continue;
     const int segment = segment_ids[next - 1];
     if (segment_ids[next] != segment) continue;
-    if (segment_starts[segment] < tile * kTile) continue;  // it began in an earlier tile, which joins it
+    const int64_t tile = segment_starts[segment] / kTile;  // where it begins
     const int64_t last = (static_cast<int64_t>(segment_starts[segment + 1]) - 1) / kTile;
+    if ((last - tile > kLongTiles) != is_long) continue;
+    // (a segment that began in an earlier tile is joined by that one's wavefront, or the workgroup of the first kLongTiles-th
+    // tile from there on; the conditions hold for a whole workgroup where the barriers are)
+    if (is_long ? at - tile >= kLongTiles : at != tile) continue;
     for (int v0 = 0; v0 < D / VEC; v0 += kWave) {
       const int chunks = min(kWave, D / VEC - v0);
       const int groups = kWave / chunks;
@@ -379,25 +414,9 @@ __global__ __launch_bounds__(kBlockThreads) void table_norm_join_kernel(
       A sum[VEC];
 #pragma unroll
       for (int k = 0; k < VEC; ++k) sum[k] = A(0);
-      if (r < groups) {
-        // (eight partial rows are requested before the first is added)
-        for (int64_t t0 = tile + r; t0 <= last; t0 += groups * kAhead) {
-          A part[kAhead][VEC];
-#pragma unroll
-          for (int a = 0; a < kAhead; ++a) {
-            const int64_t t = min(t0 + a * groups, last);
-            const A *row = partial_rows + (2 * t + (t == tile ? 1 : 0)) * D + col;
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) part[a][k] = row[k];
-          }
-#pragma unroll
-          for (int a = 0; a < kAhead; ++a) {
-            const bool real = t0 + a * groups <= last;
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) sum[k] += real ? part[a][k] : A(0);
-          }
-        }
-      }
+      if (r < groups)
+        add_partial_rows<VEC, A>(partial_rows, D, tile, tile + (is_long ? wave * groups : 0) + r,
+                                 is_long ? groups * kWavesPerBlock : groups, last, col, sum);
       for (int g = 1; g < groups; ++g) {
         const int from = min(lane + g * chunks, kWave - 1);
 #pragma unroll
@@ -406,7 +425,19 @@ __global__ __launch_bounds__(kBlockThreads) void table_norm_join_kernel(
           if (r == 0) sum[k] += o;
         }
       }
-      if (r == 0) {
+      if (is_long) {
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) s_part[wave][lane][k] = sum[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          sum[k] = A(0);
+#pragma unroll
+          for (int w = 0; w < kWavesPerBlock; ++w) sum[k] += s_part[w][lane][k];
+        }
+      }
+      if (r == 0 && (!is_long || wave == 0)) {
 #pragma unroll
         for (int k = 0; k < VEC; ++k) squares += static_cast<double>(sum[k]) * static_cast<double>(sum[k]);
       }
@@ -654,6 +685,19 @@ struct TableCall {
   hipStream_t stream;
 };
 
+// Workgroups that join: a tile per wavefront, or one workgroup for what it does in the time of a launch; and those for the
+// long segments behind them.
+struct JoinGrid {
+  int joins;
+  int64_t blocks;
+};
+JoinGrid join_grid(int64_t tiles) {
+  JoinGrid g;
+  g.joins = tiles <= kFewTiles ? 1 : static_cast<int>(std::min<int64_t>(ceil_div(tiles, kWavesPerBlock), kJoinBlocks));
+  g.blocks = g.joins + (tiles > kLongTiles ? ceil_div(tiles, kLongTiles) : 0);
+  return g;
+}
+
 // Returns the number of partial sums left, 0 if the norm is written.
 template <typename T, int VEC> unsigned launch_table(const TableCall &c, int64_t tiles, int column_blocks) {
   using A = typename AccOf<T>::type;
@@ -667,11 +711,11 @@ template <typename T, int VEC> unsigned launch_table(const TableCall &c, int64_t
   else
     TBE_LAUNCH("table_norm_tiles", c.stream, (table_norm_tiles_kernel<T, VEC, false>), grid, block, grad, psw,
                c.positions_sorted, c.grad_rows, c.segment_ids, c.n, c.D, tiles, per_xcd, rows, c.tile_sums);
-  // a tile per wavefront, or one workgroup for what that can do in the time of a launch
-  const unsigned join = tiles <= kFewTiles ? 1 : static_cast<unsigned>(std::min<int64_t>(ceil_div(tiles, kWavesPerBlock), kJoinBlocks));
-  TBE_LAUNCH("table_norm_join", c.stream, (table_norm_join_kernel<T, VEC>), dim3(join), block, c.segment_ids,
-             c.segment_starts, c.n, c.D, tiles, rows, c.tile_sums, column_blocks, c.partial, c.norm, c.f64);
-  return join == 1 ? 0 : join;
+  const JoinGrid join = join_grid(tiles);
+  TBE_LAUNCH("table_norm_join", c.stream, (table_norm_join_kernel<T, VEC>), dim3(static_cast<unsigned>(join.blocks)), block,
+             c.segment_ids, c.segment_starts, c.n, c.D, tiles, join.joins, rows, c.tile_sums, column_blocks, c.partial,
+             c.norm, c.f64);
+  return join.blocks == 1 ? 0 : static_cast<unsigned>(join.blocks);
 }
 
 }  // namespace
@@ -758,7 +802,7 @@ extern "C" int tbe_table_gradient_norm(const void *grad_output, int32_t dtype, i
   // The update's queues and partial rows are not in use between a plan and its update: the tiles' sums go to the
   // chunk records' room, the partial rows (two per kTile positions, like the update's) to their own.
   static_assert(kTile == kChunkLen, "two partial rows per tile fit the update's");
-  const int64_t join_parts = std::min<int64_t>(ceil_div(tiles, kWavesPerBlock), kJoinBlocks);
+  const int64_t join_parts = join_grid(tiles).blocks;
   const uint64_t sums = static_cast<uint64_t>(tiles * column_blocks + join_parts) * sizeof(double);
   if (sums > l.partial_sums - l.chunk_segments || column_blocks > 65535)
     return fail(TBE_ERR_UNSUPPORTED, "%s: rows of %d elements are too wide", name, D);

@@ -286,7 +286,10 @@ TABLES = [dict(T=1, E=9, D=8, B=1, L=1, ragged=False), dict(T=1, E=1, D=64, B=25
           dict(T=3, E=1000, D=100, B=50, L=9), dict(T=5, E=400, D=12, B=64, L=20, zipf=1.3),
           dict(T=2, E=50, D=4, B=300, L=10, zipf=1.1), dict(T=4, E=2000, D=260, B=100, L=12, zipf=1.2),
           dict(T=2, E=30, D=1028, B=40, L=30), dict(T=1, E=5000, D=64, B=4096, L=20, zipf=1.05),
-          dict(T=1, E=100, D=36, B=512, L=64, zipf=1.5), dict(T=3, E=20, D=2056, B=10, L=70)]
+          dict(T=1, E=100, D=36, B=512, L=64, zipf=1.5), dict(T=3, E=20, D=2056, B=10, L=70),
+          # rows of tens of thousands of lookups: segments of more than 64 tiles, alone, at both ends and side by side
+          dict(T=1, E=1, D=64, B=700, L=60, ragged=False), dict(T=2, E=2, D=24, B=1024, L=60),
+          dict(T=1, E=30, D=264, B=500, L=90, zipf=2.0)]
 
 
 @pytest.mark.parametrize("shape", TABLES, ids=lambda s: "T%(T)d_E%(E)d_D%(D)d_B%(B)d_L%(L)d" % s)
