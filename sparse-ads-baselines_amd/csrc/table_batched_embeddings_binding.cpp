@@ -109,9 +109,16 @@ struct HeldWorkspace {
   std::shared_ptr<std::mutex> busy = std::make_shared<std::mutex>();
   uint64_t last_use = 0;
 };
-static std::mutex g_workspaces_mutex;
-static std::map<std::pair<int, void *>, HeldWorkspace> g_workspaces;
-static uint64_t g_workspace_clock = 0;
+struct Scratch {
+  at::Tensor tensor;
+  std::shared_ptr<std::mutex> busy;
+  std::unique_lock<std::mutex> lock;
+  void *data() const { return tensor.data_ptr(); }
+  uint64_t bytes() const { return static_cast<uint64_t>(tensor.numel()); }
+};
+std::mutex g_workspaces_mutex;
+std::map<std::pair<int, void *>, HeldWorkspace> g_workspaces;
+uint64_t g_workspace_clock = 0;
 
 Scratch workspace(const at::Tensor &like, uint64_t bytes) {
   const std::pair<int, void *> key{static_cast<int>(like.get_device()), stream_of(like)};

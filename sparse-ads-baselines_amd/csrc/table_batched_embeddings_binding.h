@@ -3,8 +3,7 @@
 
 #include <torch/extension.h>
 
-#include <memory>
-#include <mutex>
+#include <utility>
 
 #include "tbe_hip.h"
 
@@ -30,16 +29,6 @@ void check_state(const at::Tensor &optimizer_state, const at::Tensor &weights);
 int32_t dtype_code(const at::Tensor &t);
 int64_t max_table_rows(const at::Tensor &starts_tensor, int64_t total_rows);
 std::pair<uint64_t, uint64_t> rounding_stream(const at::Tensor &t);
-
-// The scratch tensor of the current stream, held until the object goes.
-struct Scratch {
-  at::Tensor tensor;
-  std::shared_ptr<std::mutex> busy;
-  std::unique_lock<std::mutex> lock;
-  void *data() const { return tensor.data_ptr(); }
-  uint64_t bytes() const { return static_cast<uint64_t>(tensor.numel()); }
-};
-Scratch workspace(const at::Tensor &like, uint64_t bytes);
 
 // Expert routing, gradient clipping and the clipped table updates (table_batched_embeddings_training.cpp).
 void bind_training(pybind11::module &m);

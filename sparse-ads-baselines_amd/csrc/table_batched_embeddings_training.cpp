@@ -3,8 +3,8 @@
 // autograd; the kernels are in the library.  The smallest calls are bound by what the host does for them,
 // which is why these operators live here and not in the ctypes module.
 //
-// Scratch memory that a call needs comes from PyTorch's allocator for that call alone, except for the sort
-// workspace of a clipped table update, which is the stream's like that of every other update.
+// Scratch memory that a call needs comes from PyTorch's allocator for that call alone: calls on different streams, and
+// graphs captured on one stream and replayed on several, share none of it.
 #include "table_batched_embeddings_binding.h"
 
 #include <torch/csrc/autograd/custom_function.h>
@@ -315,15 +315,16 @@ struct TableClip {
 TableClip plan_and_clip(const at::Tensor &grad_output, const at::Tensor &weights, const at::Tensor &table_offsets,
                         const at::Tensor &indices, const at::Tensor &offsets,
                         const c10::optional<at::Tensor> &indice_weights, const Shape &s, int32_t dtype, double max_norm,
-                        const Scratch &ws) {
+                        const at::Tensor &ws) {
   const bool f64 = weights.scalar_type() == at::kDouble;
   TableClip clip{at::empty_like(grad_output), empty_norm(weights, f64)};
   void *stream = stream_of(weights);
+  const uint64_t bytes = static_cast<uint64_t>(ws.numel());
   check(tbe_plan_batch(table_offsets.data_ptr<int32_t>(), s.T, indices.data_ptr<int32_t>(), s.n,
                        offsets.data_ptr<int32_t>(), s.B, s.rows, max_table_rows(table_offsets, s.rows), s.D, dtype,
-                       ws.data(), ws.bytes(), stream));
-  check(tbe_table_gradient_norm(grad_output.data_ptr(), dtype, s.D, s.T, s.B, s.n, ptr(indice_weights), ws.data(),
-                                ws.bytes(), clip.norm.data_ptr(), norm_code(f64), stream));
+                       ws.data_ptr(), bytes, stream));
+  check(tbe_table_gradient_norm(grad_output.data_ptr(), dtype, s.D, s.T, s.B, s.n, ptr(indice_weights), ws.data_ptr(),
+                                bytes, clip.norm.data_ptr(), norm_code(f64), stream));
   const void *gradient = grad_output.data_ptr();
   void *output = clip.clipped.data_ptr();
   const int64_t numel = grad_output.numel();
@@ -331,10 +332,10 @@ TableClip plan_and_clip(const at::Tensor &grad_output, const at::Tensor &weights
   return clip;
 }
 
-uint64_t plan_bytes(const Shape &s, int32_t dtype) {
+at::Tensor plan_scratch(const at::Tensor &weights, const Shape &s, int32_t dtype) {
   tbe_workspace_layout_t layout;
   check(tbe_backward_workspace_layout(s.n, s.D, dtype, s.T, &layout));
-  return layout.total_bytes;
+  return at::empty({static_cast<int64_t>(layout.total_bytes)}, weights.options().dtype(at::kByte));
 }
 
 std::tuple<at::Tensor, at::Tensor> clip_table_gradient(at::Tensor grad_output, at::Tensor weights,
@@ -346,7 +347,7 @@ std::tuple<at::Tensor, at::Tensor> clip_table_gradient(at::Tensor grad_output, a
   TORCH_CHECK(max_norm >= 0.0, "max_norm must not be negative");
   const int32_t dtype = dtype_code(weights);
   c10::DeviceGuard guard(weights.device());
-  const Scratch ws = workspace(weights, plan_bytes(s, dtype));
+  const at::Tensor ws = plan_scratch(weights, s, dtype);
   const TableClip clip = plan_and_clip(grad_output, weights, table_offsets, indices, offsets, indice_weights, s, dtype,
                                        max_norm, ws);
   return {clip.clipped, clip.norm};
@@ -370,8 +371,8 @@ at::Tensor backward_clipped(int64_t optimizer, at::Tensor grad_output, at::Tenso
   c10::DeviceGuard guard(weights.device());
   const bool rounds = adagrad && stochastic_rounding && weights.scalar_type() == at::kHalf;
   std::pair<uint64_t, uint64_t> stream_of_bits{0, 0};
-  if (rounds) stream_of_bits = rounding_stream(weights);  // (takes the interpreter's lock: before the workspace's)
-  const Scratch ws = workspace(weights, plan_bytes(s, dtype));
+  if (rounds) stream_of_bits = rounding_stream(weights);
+  const at::Tensor ws = plan_scratch(weights, s, dtype);
   const TableClip clip = plan_and_clip(grad_output, weights, table_offsets, indices, offsets, indice_weights, s, dtype,
                                        max_norm, ws);
   // (the clipped gradient's dot products with the rows, which nobody asks for: the update writes them)
@@ -381,7 +382,7 @@ at::Tensor backward_clipped(int64_t optimizer, at::Tensor grad_output, at::Tenso
                              s.D, s.T, s.B, s.n, ptr(indice_weights), adagrad ? optimizer_state->data_ptr() : nullptr,
                              static_cast<float>(learning_rate), static_cast<float>(eps),
                              const_cast<void *>(ptr(unused)), rounds ? 1 : 0, stream_of_bits.first,
-                             stream_of_bits.second, ws.data(), ws.bytes(), stream_of(weights)));
+                             stream_of_bits.second, ws.data_ptr(), static_cast<uint64_t>(ws.numel()), stream_of(weights)));
   return clip.norm;
 }
 

@@ -26,8 +26,9 @@ namespace {
 //                           reads few counts, of four beyond
 //   more                    three: a launch in between turns an expert's counts into prefix sums over the tiles
 // (Measured, 8 / 64 / 256 experts: 8192 pairs in one workgroup of eight pairs a thread 9.1 / 10.9 / 12.9 us, in two
-// launches with four pairs a thread 9.1 / 9.7 / 10.6, with one 6.3 / 6.7 / 7.6; 262144 pairs 7.3 / 9.0 / 14.2 with one, 9.9 /
-// 11.7 / 14.1 with four; 524288: 13.1 / 15.1 / 18.0, 10.5 / 12.1 / 15.6, and three launches 12.1 / 13.9 / 15.7.)
+// launches with four pairs a thread 9.1 / 9.7 / 10.6, with one 6.3 / 6.7 / 7.6; 262144 pairs in two launches 7.3 / 9.0 / 14.2
+// with one, 9.9 / 11.7 / 14.1 with four; 524288 with four 10.5 / 12.1 / 15.6 in two, 12.1 / 13.9 / 15.7 in three, with one
+// 13.1 / 15.1 / 18.0 in three.)
 // A tile's pairs are ranked with wavefront ballots (all lanes of one expert are found with one ballot per bit of the
 // expert's number).  Pairs inside a tile are numbered (wavefront, item, lane), which the ranking keeps, so the
 // order is stable.
@@ -243,7 +244,7 @@ __device__ __forceinline__ bool is_kept(int32_t place, int32_t kept) {
   return static_cast<uint32_t>(place) < static_cast<uint32_t>(kept);
 }
 __device__ __forceinline__ int32_t rows_kept(const int32_t *kept_rows, int64_t pairs) {
-  return static_cast<int32_t>(min(static_cast<int64_t>(*kept_rows), pairs));
+  return static_cast<int32_t>(max(int64_t{0}, min(static_cast<int64_t>(*kept_rows), pairs)));
 }
 
 // U: what is moved per lane (Words16, or one element of 2, 4 or 8 bytes)

@@ -399,3 +399,40 @@ def test_captured_clipped_table_step():
         eager_norm = step(eager, idx.clone(), go.clone())
         torch.cuda.synchronize()
         assert torch.equal(norm, eager_norm) and torch.equal(w, eager)
+
+
+def test_graphs_captured_on_one_stream_replayed_on_two():
+    """The scratch memory of a call is its graph's own: two graphs captured on one stream may run at once."""
+    p = make_problem(19, T=2, E=400, D=32, B=256, L=30, dtype=np.float32, zipf=1.3)
+    table_offsets, off = dev(p["table_offsets"]), dev(p["offsets"])
+    w = dev(p["weights"])
+    inputs = [(dev(p["indices"]), dev(p["grad_output"])),
+              (torch.randint_like(dev(p["indices"]), 0, 400), torch.randn_like(dev(p["grad_output"])))]
+    lists = [make_list(40, [70000, 501], F32, 1)[0], make_list(41, [70000, 501], F32, 1)[0]]
+
+    def step(i):
+        idx, go = inputs[i]
+        return ops.clip_table_gradient(go, w, table_offsets, idx, off, 2.0) + (
+            ops.clip_gradients(lists[i], 1.0, out=[torch.empty_like(t) for t in lists[i]]),)
+
+    eager = [step(0), step(1)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(0)
+    torch.cuda.synchronize()
+    graphs, captured = [], []
+    for i in (0, 1):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            captured.append(step(i))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        torch.cuda.synchronize()
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for got, want in zip(captured, eager):
+            assert all(torch.equal(a, b) for a, b in zip(got, want))

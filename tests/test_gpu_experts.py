@@ -300,6 +300,9 @@ def test_places_out_of_range_are_left_alone():
                                                       torch.ones(2, 2, device=DEV))
     assert torch.equal(grad_rows[:2], torch.ones(2, 4, device=DEV))
     assert grad_w.tolist() == [[6.0, 0.0], [0.0, 22.0]]
+    offsets = torch.tensor([0, -3], dtype=torch.int32, device=DEV)  # and less than none
+    assert not ops.expert_combine(rows, places, offsets).any()
+    assert not ops.expert_dispatch(rows[:2], places, offsets)[:2].any()
 
 
 def _layer(x, ids, w, scale, experts):
