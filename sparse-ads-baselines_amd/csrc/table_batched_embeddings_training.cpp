@@ -9,6 +9,7 @@
 
 #include <torch/csrc/autograd/custom_function.h>
 
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 
 #include <limits>
@@ -30,6 +31,20 @@ int32_t float_code(const at::Tensor &t, const char *name) {
     default: TORCH_CHECK(false, name, " must be float16, bfloat16, float32 or float64");
   }
   return -1;
+}
+
+// An uninitialised tensor on the device of `like`, straight from the allocator (a third of the host time of a call
+// through the dispatcher, which would end up there).
+at::Tensor empty_on(const at::Tensor &like, at::IntArrayRef sizes, at::ScalarType type) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt));
+}
+
+// Part of `whole` as a tensor of its own: several outputs of one call share an allocation.
+at::Tensor part_of(const at::Tensor &whole, int64_t offset, at::IntArrayRef sizes) {
+  at::Tensor part = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), whole.dtype());
+  part.unsafeGetTensorImpl()->set_storage_offset(offset);
+  part.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  return part;
 }
 
 // ------------------------------------------------------------------------------ expert routing
@@ -82,14 +97,16 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> expert_plan(at::Tensor expert_ids
               num_experts, ")");
   c10::DeviceGuard guard(expert_ids.device());
   expert_ids = expert_ids.contiguous();
-  const auto ints = expert_ids.options().dtype(at::kInt);
-  at::Tensor expert_offsets = at::empty({num_experts + 1}, ints);
-  at::Tensor order = at::empty({pairs}, ints);
-  at::Tensor places = at::empty(expert_ids.sizes(), ints);
+  // places, order, expert_offsets, each from a 64-byte boundary on
+  const int64_t padded = (pairs + 15) / 16 * 16;
+  const at::Tensor whole = empty_on(expert_ids, {2 * padded + num_experts + 1}, at::kInt);
+  at::Tensor places = part_of(whole, 0, expert_ids.sizes());
+  at::Tensor order = part_of(whole, padded, {pairs});
+  at::Tensor expert_offsets = part_of(whole, 2 * padded, {num_experts + 1});
   const uint64_t bytes = tbe_expert_plan_workspace_bytes(pairs, static_cast<int32_t>(num_experts));
   // (a call of its own scratch: two graphs captured on one stream do not share it)
   at::Tensor scratch;
-  if (bytes > 0) scratch = at::empty({static_cast<int64_t>(bytes)}, expert_ids.options().dtype(at::kByte));
+  if (bytes > 0) scratch = empty_on(expert_ids, {static_cast<int64_t>(bytes)}, at::kByte);
   check(tbe_expert_plan(expert_ids.data_ptr(), static_cast<int32_t>(expert_ids.element_size()), pairs,
                         static_cast<int32_t>(num_experts), expert_offsets.data_ptr<int32_t>(),
                         order.data_ptr<int32_t>(), places.data_ptr<int32_t>(), bytes > 0 ? scratch.data_ptr() : nullptr,
@@ -102,7 +119,7 @@ at::Tensor dispatch(const at::Tensor &tokens_in, const at::Tensor &places, const
   const Plan p = check_plan(places, expert_offsets, tokens.device());
   const int32_t dtype = float_code(tokens, "tokens");
   c10::DeviceGuard guard(tokens.device());
-  at::Tensor rows = at::empty({p.tokens * p.choices, tokens.size(1)}, tokens.options());
+  at::Tensor rows = empty_on(tokens, {p.tokens * p.choices, tokens.size(1)}, tokens.scalar_type());
   check(tbe_expert_dispatch(tokens.data_ptr(), row_stride(tokens), dtype, p.tokens, p.choices, p.experts, tokens.size(1),
                             places.data_ptr<int32_t>(), expert_offsets.data_ptr<int32_t>(), rows.data_ptr(),
                             stream_of(tokens)));
@@ -117,7 +134,7 @@ at::Tensor combine(const at::Tensor &rows_in, const at::Tensor &places, const at
   c10::optional<at::Tensor> weights;
   if (weights_in.has_value()) weights = check_gates(*weights_in, rows, places);
   c10::DeviceGuard guard(rows.device());
-  at::Tensor output = at::empty({p.tokens, rows.size(1)}, rows.options());
+  at::Tensor output = empty_on(rows, {p.tokens, rows.size(1)}, rows.scalar_type());
   check(tbe_expert_combine(rows.data_ptr(), row_stride(rows), dtype, p.tokens, p.choices, p.experts, rows.size(1),
                            places.data_ptr<int32_t>(), expert_offsets.data_ptr<int32_t>(), ptr(weights),
                            weights.has_value() ? float_code(*weights, "weights") : dtype, output.data_ptr(),
@@ -140,8 +157,8 @@ std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>> combine_backwar
   const at::Tensor grad = check_rows(grad_in, "grad_output", p.tokens);
   c10::DeviceGuard guard(rows.device());
   c10::optional<at::Tensor> grad_rows, grad_weights;
-  if (want_rows) grad_rows = at::empty({rows.size(0), rows.size(1)}, rows.options());
-  if (want_weights) grad_weights = at::empty(places.sizes(), weights.options());
+  if (want_rows) grad_rows = empty_on(rows, {rows.size(0), rows.size(1)}, rows.scalar_type());
+  if (want_weights) grad_weights = empty_on(rows, places.sizes(), weights.scalar_type());
   if (!want_rows && !want_weights) return {grad_rows, grad_weights};
   check(tbe_expert_combine_backward(
       grad.data_ptr(), row_stride(grad), rows.data_ptr(), row_stride(rows), dtype, p.tokens, p.choices, p.experts,
@@ -268,7 +285,7 @@ GradientList check_gradients(const TensorSequence &gradients, const TensorSequen
 }
 
 at::Tensor empty_norm(const at::Tensor &like, bool f64) {
-  return at::empty({}, like.options().dtype(f64 ? at::kDouble : at::kFloat));
+  return empty_on(like, {}, f64 ? at::kDouble : at::kFloat);
 }
 int32_t norm_code(bool f64) { return f64 ? TBE_DTYPE_F64 : TBE_DTYPE_F32; }
 
@@ -279,7 +296,7 @@ at::Tensor gradient_norm(const py::object &source) {
   c10::DeviceGuard guard(first.device());
   at::Tensor norm = empty_norm(first, list.f64);
   const uint64_t bytes = tbe_gradient_norm_workspace_bytes(list.count());
-  at::Tensor scratch = at::empty({static_cast<int64_t>(bytes)}, first.options().dtype(at::kByte));
+  at::Tensor scratch = empty_on(first, {static_cast<int64_t>(bytes)}, at::kByte);
   check(tbe_gradient_norm(list.gradients.data(), list.numels.data(), list.dtypes.data(), list.count(), norm.data_ptr(),
                           norm_code(list.f64), scratch.data_ptr(), bytes, stream_of(first)));
   return norm;
@@ -295,7 +312,7 @@ at::Tensor clip_gradients(const py::object &source, double max_norm, const py::o
   c10::DeviceGuard guard(first.device());
   at::Tensor norm = empty_norm(first, list.f64);
   const uint64_t bytes = tbe_gradient_norm_workspace_bytes(list.count());
-  at::Tensor scratch = at::empty({static_cast<int64_t>(bytes)}, first.options().dtype(at::kByte));
+  at::Tensor scratch = empty_on(first, {static_cast<int64_t>(bytes)}, at::kByte);
   check(tbe_clip_gradients(list.gradients.data(), list.outputs.data(), list.numels.data(), list.dtypes.data(),
                            list.count(), max_norm, norm.data_ptr(), norm_code(list.f64), scratch.data_ptr(), bytes,
                            stream_of(first)));
@@ -317,7 +334,7 @@ TableClip plan_and_clip(const at::Tensor &grad_output, const at::Tensor &weights
                         const c10::optional<at::Tensor> &indice_weights, const Shape &s, int32_t dtype, double max_norm,
                         const at::Tensor &ws) {
   const bool f64 = weights.scalar_type() == at::kDouble;
-  TableClip clip{at::empty_like(grad_output), empty_norm(weights, f64)};
+  TableClip clip{empty_on(grad_output, grad_output.sizes(), grad_output.scalar_type()), empty_norm(weights, f64)};
   void *stream = stream_of(weights);
   const uint64_t bytes = static_cast<uint64_t>(ws.numel());
   check(tbe_plan_batch(table_offsets.data_ptr<int32_t>(), s.T, indices.data_ptr<int32_t>(), s.n,
@@ -335,7 +352,7 @@ TableClip plan_and_clip(const at::Tensor &grad_output, const at::Tensor &weights
 at::Tensor plan_scratch(const at::Tensor &weights, const Shape &s, int32_t dtype) {
   tbe_workspace_layout_t layout;
   check(tbe_backward_workspace_layout(s.n, s.D, dtype, s.T, &layout));
-  return at::empty({static_cast<int64_t>(layout.total_bytes)}, weights.options().dtype(at::kByte));
+  return empty_on(weights, {static_cast<int64_t>(layout.total_bytes)}, at::kByte);
 }
 
 std::tuple<at::Tensor, at::Tensor> clip_table_gradient(at::Tensor grad_output, at::Tensor weights,
