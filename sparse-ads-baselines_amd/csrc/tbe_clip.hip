@@ -158,9 +158,9 @@ __device__ __forceinline__ void chunk_scaled(const Piece<T> &p, typename AccOf<T
   if (thread < p.head) dst[thread - p.head] = static_cast<T>(static_cast<A>(src[thread - p.head]) * scale);
 }
 
-__device__ __forceinline__ void store_norm(void *norm, int f64, double sum) {
-  if (f64) *static_cast<double *>(norm) = sqrt(sum);
-  else *static_cast<float *>(norm) = static_cast<float>(sqrt(sum));
+__device__ __forceinline__ void store_norm(void *norm, int f64, double value) {
+  if (f64) *static_cast<double *>(norm) = value;
+  else *static_cast<float *>(norm) = static_cast<float>(value);
 }
 
 // The norm is rounded once, to the type it is stored in; the scale is formed in 64 bits from it.
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(kWideThreads) void norm_finish_kernel(const double 
   double sum = 0.0;
   for (int64_t i = threadIdx.x; i < count; i += kWideThreads) sum += partial[i];
   sum = block_sum<kWideThreads / kWave>(sum);
-  if (threadIdx.x == 0) store_norm(norm, f64, sum);
+  if (threadIdx.x == 0) store_norm(norm, f64, sqrt(sum));
 }
 
 // A vector per thread and chunk (reading and writing want many short requests: 427 us with four vectors a thread where
@@ -203,6 +203,23 @@ __global__ __launch_bounds__(kWideThreads) void scale_kernel(L list, const void 
     chunk_scaled<T, kWideThreads, 1, STREAM_IN, STREAM_OUT>(piece_of_chunk<T>(list, chunk), scale, threadIdx.x);
 }
 
+// The same behind a sum over at most kWideThreads workgroups: every workgroup adds up the partial sums itself, in the
+// same order, and the first one writes the norm.  That takes about as long as it is spared, a launch, while the workgroups
+// all run at once (two per compute unit).
+constexpr int kJoinedChunks = 512;
+template <typename T, typename L>
+__global__ __launch_bounds__(kWideThreads) void scale_joined_kernel(L list, const double *__restrict__ partial, int count,
+                                                                    void *norm, int f64, double max_norm) {
+  using A = typename AccOf<T>::type;
+  const double root = sqrt(block_sum<kWideThreads / kWave>(static_cast<int>(threadIdx.x) < count ? partial[threadIdx.x] : 0.0));
+  const double n = f64 ? root : static_cast<double>(static_cast<float>(root));
+  if (blockIdx.x == 0 && threadIdx.x == 0) store_norm(norm, f64, root);
+  const A scale = static_cast<A>(clip_scale(n, max_norm));
+  if (!L::kPairs && scale == A(1)) return;
+  for (int chunk = blockIdx.x; chunk < list.chunks; chunk += gridDim.x)
+    chunk_scaled<T, kWideThreads, 1, false, false>(piece_of_chunk<T>(list, chunk), scale, threadIdx.x);
+}
+
 // Few chunks: norm and scaling in one workgroup, a wavefront per chunk.
 constexpr int kFewChunks = 32;
 template <typename T, typename L>
@@ -216,9 +233,10 @@ __global__ __launch_bounds__(kWideThreads) void clip_few_kernel(L list, int scal
   for (int chunk = wave; chunk < list.chunks; chunk += kWaves)
     sum += chunk_squares<T, kWave, 8, false>(piece_of_chunk<T>(list, chunk), lane);
   sum = block_sum<kWaves>(sum);
-  if (threadIdx.x == 0) store_norm(norm, f64, sum);
+  const double root = sqrt(sum);
+  if (threadIdx.x == 0) store_norm(norm, f64, root);
   if (!scaled) return;
-  const double n = f64 ? sqrt(sum) : static_cast<double>(static_cast<float>(sqrt(sum)));
+  const double n = f64 ? root : static_cast<double>(static_cast<float>(root));
   const A scale = static_cast<A>(clip_scale(n, max_norm));
   if (!L::kPairs && scale == A(1)) return;
   for (int chunk = wave; chunk < list.chunks; chunk += kWaves)
@@ -445,7 +463,7 @@ __global__ __launch_bounds__(kBlockThreads) void table_norm_join_kernel(
   }
   squares = block_sum<kWavesPerBlock>(squares);
   if (threadIdx.x != 0) return;
-  if (gridDim.x == 1) store_norm(norm, f64, squares);  // (no more launches: this is all of it)
+  if (gridDim.x == 1) store_norm(norm, f64, sqrt(squares));  // (no more launches: this is all of it)
   else partial[blockIdx.x] = squares;
 }
 
@@ -591,8 +609,8 @@ uint64_t total_bytes(const ListCall &c) {
 // streamed (1.2 GB squared and scaled: 558 us, 619 with plain accesses; 240 MB: 116 and 99 the other way round).
 bool streams(uint64_t bytes) { return bytes > (uint64_t{256} << 20); }
 
-void launch_norm(const ListCall &c, void *workspace, void *norm, int32_t norm_dtype, hipStream_t s) {
-  double *partial = static_cast<double *>(workspace);
+// The partial sums of all lists; returns their number.
+int64_t launch_squares(const ListCall &c, double *partial, hipStream_t s) {
   int64_t used = 0;
   const bool stream = streams(total_bytes(c));
   for (const int32_t dtype : kDtypes) {
@@ -606,6 +624,12 @@ void launch_norm(const ListCall &c, void *workspace, void *norm, int32_t norm_dt
       used += grid.x;
     });
   }
+  return used;
+}
+
+void launch_norm(const ListCall &c, void *workspace, void *norm, int32_t norm_dtype, hipStream_t s) {
+  double *partial = static_cast<double *>(workspace);
+  const int64_t used = launch_squares(c, partial, s);
   TBE_LAUNCH("gradient_norm", s, norm_finish_kernel, dim3(1), dim3(kWideThreads), partial, used, norm,
              norm_dtype == TBE_DTYPE_F64 ? 1 : 0);
 }
@@ -633,28 +657,56 @@ void launch_scale(const ListCall &c, double max_norm, const void *norm, int32_t 
   }
 }
 
-// A list of one type and few chunks goes through one workgroup in one launch: whether it did.  (Eleven fp32 tensors of
-// 60001 elements in all, 26 chunks.)
-bool launch_few(const ListCall &c, double max_norm, void *norm, int32_t norm_dtype, hipStream_t s) {
-  int32_t dtype = -1;
+// What a call's lists come to, for the forms that take one list.
+struct Lists {
+  int32_t dtype = -1;     // -1: no elements; -2: several types
   int64_t tensors = 0, chunks = 0;
-  const bool same = !c.outputs || in_place(c);
+  bool same;              // nothing is written, or in place
+};
+Lists count_lists(const ListCall &c) {
+  Lists l;
+  l.same = !c.outputs || in_place(c);
   for (int32_t i = 0; i < c.count; ++i) {
     if (c.numels[i] == 0) continue;
-    if (dtype >= 0 && c.dtypes[i] != dtype) return false;
-    dtype = c.dtypes[i];
-    ++tensors;
-    chunks += chunks_of(c.numels[i], reinterpret_cast<uint64_t>(same ? c.gradients[i] : c.outputs[i]), dtype).count;
-    if (tensors > kPairTensors || chunks > kFewChunks) return false;
+    l.dtype = l.dtype == -1 || l.dtype == c.dtypes[i] ? c.dtypes[i] : -2;
+    ++l.tensors;
+    l.chunks += chunks_of(c.numels[i], reinterpret_cast<uint64_t>(l.same ? c.gradients[i] : c.outputs[i]), c.dtypes[i]).count;
   }
-  if (tensors == 0) return false;
-  with_type(dtype, [&](auto t) {
-    const auto launch = [&](const auto &list) {
+  return l;
+}
+
+// f(list) for the one list of a call whose tensors fit it.
+template <typename F> void for_one_list(const ListCall &c, const Lists &l, F &&f) {
+  if (l.same) for_lists<ReadList>(c, l.dtype, f);
+  else for_lists<PairList>(c, l.dtype, f);
+}
+
+// Norm (c.outputs null) or norm and scaling of one list of at most kFewChunks chunks, in one launch; whether it was one.
+bool launch_few(const ListCall &c, const Lists &l, double max_norm, void *norm, int32_t norm_dtype, hipStream_t s) {
+  if (l.dtype < 0 || l.chunks > kFewChunks) return false;
+  with_type(l.dtype, [&](auto t) {
+    for_one_list(c, l, [&](const auto &list) {
       TBE_LAUNCH("gradient_clip_few", s, (clip_few_kernel<decltype(t), std::decay_t<decltype(list)>>), dim3(1),
                  dim3(kWideThreads), list, c.outputs ? 1 : 0, norm, norm_dtype == TBE_DTYPE_F64 ? 1 : 0, max_norm);
-    };
-    if (same) for_lists<ReadList>(c, dtype, launch);
-    else for_lists<PairList>(c, dtype, launch);
+    });
+  });
+  return true;
+}
+
+// Norm and scaling of one list of at most kJoinedChunks chunks, in two launches; whether it was one.  (100 tensors of 100 k
+// fp32 elements in all, outputs of their own: a pass of 10.6 us, 15.1 with a launch for the norm in between.)
+bool launch_joined(const ListCall &c, const Lists &l, double max_norm, void *workspace, void *norm, int32_t norm_dtype,
+                   hipStream_t s) {
+  if (l.dtype < 0 || l.chunks > kJoinedChunks || l.tensors > (l.same ? kListTensors : kPairTensors)) return false;
+  double *partial = static_cast<double *>(workspace);
+  const int64_t used = launch_squares(c, partial, s);
+  with_type(l.dtype, [&](auto t) {
+    using T = decltype(t);
+    for_one_list(c, l, [&](const auto &list) {
+      TBE_LAUNCH("gradient_scale", s, (scale_joined_kernel<T, std::decay_t<decltype(list)>>),
+                 dim3(static_cast<unsigned>(list.chunks)), dim3(kWideThreads), list, partial, static_cast<int>(used), norm,
+                 norm_dtype == TBE_DTYPE_F64 ? 1 : 0, max_norm);
+    });
   });
   return true;
 }
@@ -736,7 +788,7 @@ extern "C" int tbe_gradient_norm(const void *const *gradients, const int64_t *nu
   if (int rc = check_norm(name, norm, norm_dtype)) return rc;
   if (int rc = check_workspace(name, num_tensors, workspace, workspace_bytes)) return rc;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (!launch_few(c, 0.0, norm, norm_dtype, s)) launch_norm(c, workspace, norm, norm_dtype, s);
+  if (!launch_few(c, count_lists(c), 0.0, norm, norm_dtype, s)) launch_norm(c, workspace, norm, norm_dtype, s);
   return check_launch(name);
 }
 
@@ -766,7 +818,9 @@ extern "C" int tbe_clip_gradients(const void *const *gradients, void *const *out
   if (int rc = check_workspace(name, num_tensors, workspace, workspace_bytes)) return rc;
   if (int rc = check_overlap(name, c)) return rc;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (!launch_few(c, max_norm, norm, norm_dtype, s)) {
+  const Lists l = count_lists(c);
+  if (!launch_few(c, l, max_norm, norm, norm_dtype, s) &&
+      !launch_joined(c, l, max_norm, workspace, norm, norm_dtype, s)) {
     launch_norm(c, workspace, norm, norm_dtype, s);
     launch_scale(c, max_norm, norm, norm_dtype, s);
   }
