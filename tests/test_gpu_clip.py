@@ -436,3 +436,45 @@ def test_graphs_captured_on_one_stream_replayed_on_two():
         torch.cuda.synchronize()
         for got, want in zip(captured, eager):
             assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_whole_training_step_with_experts_and_clipping():
+    """Bags that clip their tables' gradient, an expert layer on top, dense gradients clipped together: the step is the
+    unclipped one with every gradient scaled by its own norm's factor."""
+    T, E, D, B, experts, choices = 3, 150, 32, 64, 5, 2
+    p = make_problem(23, T, E, D, B, 8, np.float32, zipf=1.3)
+    ids = torch.randint(-1, experts, (B * T, choices), device=DEV, generator=torch.Generator(device=DEV).manual_seed(2))
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    matrices0 = torch.randn(experts, D, D, device=DEV, generator=gen) * 0.2
+    gates0 = torch.rand(B * T, choices, device=DEV, generator=gen)
+    lr = 0.5
+
+    def step(table_limit, dense_limit):
+        bags = ops.TableBatchedEmbeddingBags(T, E, D, optimizer=ops.Optimizer.SGD, learning_rate=lr).cuda()
+        bags.embedding_weights.data.copy_(dev(p["weights"]))
+        clip = bags.clip_gradient(table_limit)
+        matrices, gates = (torch.nn.Parameter(t.clone()) for t in (matrices0, gates0))
+        routing = ops.ExpertRouting(ids, experts)
+        rows = routing.dispatch(bags(dev(p["indices"]), dev(p["offsets"])).reshape(B * T, D))
+        bounds = routing.expert_offsets.tolist()
+        done = [torch.tanh(rows[bounds[e]:bounds[e + 1]] @ matrices[e]) for e in range(experts)]
+        y = routing.combine(torch.cat(done + [rows[bounds[-1]:]]), gates)
+        (100.0 * y).square().sum().backward()
+        norm = ops.clip_grad_norm_(list(bags.parameters()) + [matrices, gates], dense_limit)
+        moved = bags.embedding_weights.detach().double() - dev(p["weights"]).double()
+        return moved, matrices.grad.double(), gates.grad.double(), float(norm), float(clip.norm)
+
+    free = step(float("inf"), float("inf"))
+    table_norm = float(free[0].norm()) / lr  # every row moved by -lr times its gradient, but for the weights' rounding
+    assert abs(free[4] - table_norm) <= 1e-3 * table_norm
+    assert abs(free[3] - float(torch.cat([free[1].flatten(), free[2].flatten()]).norm())) <= 1e-6 * free[3]
+    table_limit, dense_limit = 0.25 * free[4], 0.4 * free[3]
+    clipped = step(table_limit, dense_limit)
+    assert clipped[3:] == free[3:]  # the same norms before scaling
+    for got, want, scale in ((clipped[0], free[0], table_limit / (free[4] + 1e-6)),
+                             (clipped[1], free[1], dense_limit / (free[3] + 1e-6)),
+                             (clipped[2], free[2], dense_limit / (free[3] + 1e-6))):
+        # three roundings of the scaled values, and for the table the rounding of both sides' weights
+        weights = 2 * 2.0 ** -24 * 0.01 * math.sqrt(got.numel()) if got is clipped[0] else 0.0
+        step_rounding = 2.0 ** -24 * (float(want.norm()) + float(got.norm()))
+        assert float((got - scale * want).norm()) <= 4 * 2.0 ** -24 * float(got.norm()) + 2 * step_rounding + weights
