@@ -466,6 +466,14 @@ extern "C" int tbe_plan_batch(const int32_t *table_offsets, int32_t T, const int
   if (!workspace || workspace_bytes < l.total_bytes)
     return fail(TBE_ERR_WORKSPACE, "%s: workspace of %llu bytes needed, %llu given", name,
                 (unsigned long long)l.total_bytes, (unsigned long long)workspace_bytes);
+  if (small_plan_serves(num_indices, T, B)) {
+    char *ws = static_cast<char *>(workspace);
+    const auto at = [&](uint64_t region) { return reinterpret_cast<int32_t *>(ws + region); };
+    const int64_t largest = max_table_rows > 0 && max_table_rows < total_rows ? max_table_rows : total_rows;
+    return plan_small(table_offsets, T, indices, num_indices, offsets, B, key_bits(largest), at(l.keys_sorted),
+                      at(l.positions_sorted), at(l.grad_rows), at(l.segment_starts), at(l.segment_ids),
+                      at(l.num_unique), static_cast<hipStream_t>(stream));
+  }
   return build_plan(l, workspace, table_offsets, T, indices, num_indices, offsets, B, total_rows,
                     max_table_rows, static_cast<hipStream_t>(stream));
 }

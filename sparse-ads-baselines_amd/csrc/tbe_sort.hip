@@ -802,6 +802,194 @@ __global__ __launch_bounds__(kBlockThreads) void segment_write_kernel(
   for (uint32_t i = threadIdx.x; i < total; i += kBlockThreads) segment_starts[base + i] = s_heads[i];
 }
 
+// ------------------------------------------------------------------ plan of a small batch
+// Gradient rows, sort and segments of up to kSmallPlan lookups in one workgroup and one launch: what the kernels above
+// write, from LDS.  They are 5 to 11 dependent launches, which is all that such a batch costs.  The pairs are sorted by
+// (table, row inside the table) in digits of at most 8 bits, with the ranking of the scatter kernel; a position's bag
+// is the last one that begins at or before it (the largest bag number over the positions up to it, bags without lookups
+// aside).  (Plan, norm and scaling of rows of 32 floats, this way and with the kernels above: 512 lookups in 2 tables of
+// 1000 rows 16.7 and 27.4 us, 2048 in 4 of 100 000 22.5 and 38.5, 4096 in one of 100 000 28.9 and 42.9, 4096 in 64 of
+// 1000, the least they need, 27.5 and 28.3.)
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanWaves = kPlanThreads / kWave;
+constexpr int kPlanBins = 256;
+constexpr int kPlanTables = 1024;      // key biases in LDS
+constexpr int kPlanPositionBits = 12;  // of a pair's payload, its position; the table above them
+static_assert(kSmallPlan <= 1 << kPlanPositionBits && kSmallPlan % kPlanThreads == 0, "payload");
+
+template <int ITEMS>
+__global__ __launch_bounds__(kPlanThreads) void plan_small_kernel(
+    const int32_t *__restrict__ table_offsets, int T, const uint32_t *__restrict__ indices, int n,
+    const int32_t *__restrict__ offsets, int B, int row_bits, int table_bits, uint32_t *__restrict__ keys_sorted,
+    int32_t *__restrict__ positions_sorted, int32_t *__restrict__ grad_rows, int32_t *__restrict__ segment_starts,
+    int32_t *__restrict__ segment_ids, int32_t *__restrict__ num_unique) {
+  constexpr int kPairs = kPlanThreads * ITEMS;
+  __shared__ uint32_t s_key[kPairs];
+  __shared__ uint32_t s_value[kPairs];  // (first: the bag that begins at a position)
+  __shared__ uint32_t s_count[kPlanWaves][kPlanBins];
+  __shared__ uint32_t s_bias[kPlanTables];
+  __shared__ uint32_t s_wave[kPlanWaves];
+  const int tid = threadIdx.x;
+  const int lane = tid & (kWave - 1);
+  const int wave = tid >> 6;
+  // this thread's pairs: position order is (wavefront, item, lane)
+  const int first = wave * (kWave * ITEMS) + lane;
+  uint32_t key[ITEMS], value[ITEMS];
+#pragma unroll
+  for (int q = 0; q < ITEMS; ++q) {
+    key[q] = first + q * kWave < n ? indices[first + q * kWave] : 0u;
+    s_value[first + q * kWave] = 0;
+  }
+  if (tid < T) s_bias[tid] = static_cast<uint32_t>(table_offsets[tid]);
+  __syncthreads();
+  for (int g = tid; g < T * B; g += kPlanThreads) {
+    const int begin = max(offsets[g], 0);
+    if (begin < min(offsets[g + 1], n)) atomicMax(&s_value[begin], static_cast<uint32_t>(g));
+  }
+  __syncthreads();
+  {
+    uint32_t last = 0;
+#pragma unroll
+    for (int q = 0; q < ITEMS; ++q) {
+      uint32_t bag = s_value[first + q * kWave];
+#pragma unroll
+      for (int d = 1; d < kWave; d <<= 1) bag = max(bag, static_cast<uint32_t>(__shfl_up(bag, d, kWave)));
+      value[q] = max(bag, last);
+      last = __shfl(value[q], kWave - 1, kWave);
+    }
+    if (lane == 0) s_wave[wave] = last;
+  }
+  __syncthreads();
+  {
+    uint32_t before = 0;
+    for (int w = 0; w < wave; ++w) before = max(before, s_wave[w]);
+#pragma unroll
+    for (int q = 0; q < ITEMS; ++q) {
+      const int p = first + q * kWave;
+      const int bag = static_cast<int>(max(value[q], before));
+      const int t = bag / B;
+      if (p < n) grad_rows[p] = (bag - t * B) * T + t;
+      value[q] = static_cast<uint32_t>(t) << kPlanPositionBits | static_cast<uint32_t>(p);
+    }
+  }
+  const int bits = row_bits + table_bits;
+  const int passes = (bits + 7) / 8;
+  for (int pass = 0, shift = 0; pass < passes; ++pass) {
+    const int width = (bits - shift + passes - pass - 1) / (passes - pass);
+    uint32_t digit[ITEMS], rank[ITEMS];
+#pragma unroll
+    for (int i = 0; i < kPlanBins / kWave; ++i) s_count[wave][lane + i * kWave] = 0;
+    // (a wavefront counts its own pairs; LDS serves one wavefront's accesses in order)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int q = 0; q < ITEMS; ++q) {
+      const bool real = first + q * kWave < n;
+      const uint64_t c = static_cast<uint64_t>(value[q] >> kPlanPositionBits) << row_bits |
+                         (key[q] & static_cast<uint32_t>((uint64_t{1} << row_bits) - 1));
+      digit[q] = static_cast<uint32_t>(c >> shift) & ((1u << width) - 1);
+      uint64_t same = __ballot(real);
+      for (int b = 0; b < width; ++b) {
+        const bool set = (digit[q] >> b) & 1;
+        const uint64_t vote = __ballot(set);
+        same &= set ? vote : ~vote;
+      }
+      rank[q] = 0;
+      if (real) {
+        const int leader = __ffsll(static_cast<unsigned long long>(same)) - 1;
+        uint32_t before = 0;
+        if (lane == leader) before = atomicAdd(&s_count[wave][digit[q]], static_cast<uint32_t>(__popcll(same)));
+        rank[q] = __shfl(before, leader, kWave) + __popcll(same & ((uint64_t{1} << lane) - 1));
+      }
+    }
+    __syncthreads();
+    // where every (digit, wavefront) begins: over the wavefronts of a digit, then over the digits
+    uint32_t total = 0, incl = 0;
+    if (tid < kPlanBins) {
+#pragma unroll
+      for (int w = 0; w < kPlanWaves; ++w) {
+        const uint32_t c = s_count[w][tid];
+        s_count[w][tid] = total;
+        total += c;
+      }
+      incl = total;
+#pragma unroll
+      for (int d = 1; d < kWave; d <<= 1) {
+        const uint32_t y = __shfl_up(incl, d, kWave);
+        if (lane >= d) incl += y;
+      }
+      if (lane == kWave - 1) s_wave[wave] = incl;
+    }
+    __syncthreads();
+    if (tid < kPlanBins) {
+      uint32_t start = incl - total;
+      for (int w = 0; w < wave; ++w) start += s_wave[w];
+#pragma unroll
+      for (int w = 0; w < kPlanWaves; ++w) s_count[w][tid] += start;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < ITEMS; ++q) {
+      if (first + q * kWave >= n) continue;
+      const uint32_t to = s_count[wave][digit[q]] + rank[q];
+      s_key[to] = key[q];
+      s_value[to] = value[q];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < ITEMS; ++q) {
+      if (first + q * kWave >= n) continue;
+      key[q] = s_key[first + q * kWave];
+      value[q] = s_value[first + q * kWave];
+    }
+    shift += width;
+  }
+  // segments: a position that begins one has another key than the position before it
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < ITEMS; ++q) {
+    const int p = first + q * kWave;
+    if (p >= n) continue;
+    key[q] += s_bias[value[q] >> kPlanPositionBits];
+    s_key[p] = key[q];
+    keys_sorted[p] = key[q];
+    positions_sorted[p] = static_cast<int32_t>(value[q] & ((1u << kPlanPositionBits) - 1));
+  }
+  __syncthreads();
+  uint32_t heads = 0;  // of the wavefront, up to an item
+  bool head[ITEMS];
+#pragma unroll
+  for (int q = 0; q < ITEMS; ++q) {
+    const int p = first + q * kWave;
+    head[q] = p < n && (p == 0 || s_key[p] != s_key[p - 1]);
+    const uint64_t vote = __ballot(head[q]);
+    value[q] = heads + __popcll(vote & (~uint64_t{0} >> (kWave - 1 - lane)));
+    heads += __popcll(vote);
+  }
+  if (lane == 0) s_wave[wave] = heads;
+  __syncthreads();
+  uint32_t before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanWaves; ++w) {
+    if (w < wave) before += s_wave[w];
+    all += s_wave[w];
+  }
+#pragma unroll
+  for (int q = 0; q < ITEMS; ++q) {
+    const int p = first + q * kWave;
+    if (p >= n) continue;
+    const int32_t id = static_cast<int32_t>(before + value[q]) - 1;
+    segment_ids[p] = id;
+    if (head[q]) segment_starts[id] = p;
+  }
+  if (tid == 0) {
+    num_unique[0] = static_cast<int32_t>(all);
+    segment_starts[all] = n;
+  } else if (tid < kNumCounters) {
+    num_unique[tid] = 0;
+  }
+}
+static_assert(kNumCounters <= kPlanThreads, "the counters are cleared by one workgroup");
+
 inline int num_seg_tiles(int64_t n) { return static_cast<int>(ceil_div(n, kSegTile)); }
 
 }  // namespace
@@ -996,6 +1184,27 @@ int find_segments(const int32_t *keys_sorted, int64_t n, int32_t *segment_starts
     TBE_LAUNCH("segment_write", stream, segment_write_kernel<false>, dim3(tiles), block, keys, n,
                tile_heads, segment_starts, segment_ids, num_unique, 0);
   return check_launch("tbe_find_segments");
+}
+
+bool small_plan_serves(int64_t n, int32_t T, int32_t B) {
+  return n > 0 && n <= kSmallPlan && T <= kPlanTables && static_cast<int64_t>(T) * B <= kSmallPlanBags;
+}
+
+int plan_small(const int32_t *table_offsets, int32_t T, const int32_t *indices, int64_t n, const int32_t *offsets,
+               int32_t B, int32_t row_bits, int32_t *keys_sorted, int32_t *positions_sorted, int32_t *grad_rows,
+               int32_t *segment_starts, int32_t *segment_ids, int32_t *num_unique, hipStream_t stream) {
+  int table_bits = 0;
+  while ((1 << table_bits) < T) ++table_bits;
+#define TBE_PLAN_SMALL(ITEMS)                                                                                      \
+  TBE_LAUNCH("plan_small", stream, plan_small_kernel<ITEMS>, dim3(1), dim3(kPlanThreads), table_offsets, T,          \
+             reinterpret_cast<const uint32_t *>(indices), static_cast<int>(n), offsets, B, row_bits, table_bits,   \
+             reinterpret_cast<uint32_t *>(keys_sorted), positions_sorted, grad_rows, segment_starts, segment_ids,  \
+             num_unique)
+  if (n <= kPlanThreads) { TBE_PLAN_SMALL(1); }
+  else if (n <= 2 * kPlanThreads) { TBE_PLAN_SMALL(2); }
+  else { TBE_PLAN_SMALL(4); }
+#undef TBE_PLAN_SMALL
+  return check_launch("tbe_plan_batch");
 }
 
 int linearize(const int32_t *table_offsets, int32_t T, const int32_t *indices,

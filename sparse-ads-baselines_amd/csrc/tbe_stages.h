@@ -46,6 +46,15 @@ int find_segments(const int32_t *keys_sorted, int64_t n, int32_t *segment_starts
                   int32_t *num_unique, int32_t *segment_ids, void *workspace, hipStream_t stream,
                   bool clear_queue_counters = false);
 
+// A batch of up to kSmallPlan lookups in up to kSmallPlanBags bags, planned in one launch: what linearize, sort_pairs and
+// find_segments (clear_queue_counters) write, bit for bit.
+constexpr int kSmallPlan = 4096;
+constexpr int64_t kSmallPlanBags = 8192;
+bool small_plan_serves(int64_t n, int32_t T, int32_t B);
+int plan_small(const int32_t *table_offsets, int32_t T, const int32_t *indices, int64_t n, const int32_t *offsets,
+               int32_t B, int32_t row_bits, int32_t *keys_sorted, int32_t *positions_sorted, int32_t *grad_rows,
+               int32_t *segment_starts, int32_t *segment_ids, int32_t *num_unique, hipStream_t stream);
+
 // Segments of more than kShortSegment occurrences leave the lane-group path and are reduced by
 // whole wavefronts in chunks of at most kChunkLen occurrences.  (Measured, fused forward + backward
 // of 5.2 M lookups: 64 tables of 100 k fp32 rows of 128, Zipf 1.05 / 32 tables of 1 M fp16 rows of
