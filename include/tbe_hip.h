@@ -652,8 +652,9 @@ TBE_API int tbe_backward_sgd_interleaved(const void *grad_output, void *weights,
  *   combine_backward  grad_rows[places[a]] = weights[a] * grad_output[t] (zeros for a dropped pair),
  *                     grad_weights[a] = <rows[places[a]], grad_output[t]> (zero for a dropped pair);
  *                     either may be NULL (without grad_weights, rows are not read and may be NULL too)
- * A place outside [0, num_rows) is treated as a dropped pair's and not written.  The calls only launch kernels
- * on `stream`; they can be captured.
+ * A place outside [0, num_rows) is treated as a dropped pair's and not written; rows that no place names are not
+ * written either, and of two pairs that name one row either may win (a plan's places name every row once).  The
+ * calls only launch kernels on `stream`; they can be captured.
  */
 #define TBE_MAX_EXPERTS 4095
 TBE_API uint64_t tbe_expert_plan_workspace_bytes(int64_t num_pairs, int32_t num_experts);

@@ -173,6 +173,11 @@ void refuse_second_derivative() {
   TORCH_CHECK(!at::GradMode::is_enabled(), "expert routing is differentiable once (create_graph=True is not served)");
 }
 
+// (nor do they carry a tangent)
+void refuse_tangent(const at::Tensor &t) {
+  TORCH_CHECK(!t._fw_grad(0).defined(), "expert routing has no forward-mode derivative");
+}
+
 struct Dispatch : torch::autograd::Function<Dispatch> {
   static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &tokens, const at::Tensor &places,
                             const at::Tensor &expert_offsets) {
@@ -209,12 +214,15 @@ struct Combine : torch::autograd::Function<Combine> {
 };
 
 at::Tensor expert_dispatch(const at::Tensor &tokens, const at::Tensor &places, const at::Tensor &expert_offsets) {
+  refuse_tangent(tokens);
   if (at::GradMode::is_enabled() && tokens.requires_grad()) return Dispatch::apply(tokens, places, expert_offsets);
   return dispatch(tokens, places, expert_offsets);
 }
 
 at::Tensor expert_combine(const at::Tensor &rows, const at::Tensor &places, const at::Tensor &expert_offsets,
                           const c10::optional<at::Tensor> &weights) {
+  refuse_tangent(rows);
+  if (weights.has_value()) refuse_tangent(*weights);
   if (at::GradMode::is_enabled() && (rows.requires_grad() || (weights.has_value() && weights->requires_grad())))
     return Combine::apply(rows, places, expert_offsets, weights);
   return combine(rows, places, expert_offsets, weights);

@@ -204,9 +204,11 @@ __global__ __launch_bounds__(kWideThreads) void scale_kernel(L list, const void 
 }
 
 // The same behind a sum over at most kWideThreads workgroups: every workgroup adds up the partial sums itself, in the
-// same order, and the first one writes the norm.  That takes about as long as it is spared, a launch, while the workgroups
-// all run at once (two per compute unit).
+// same order, and the first one writes the norm, in place of a launch in between.  For lists whose workgroups all run at
+// once, two per compute unit.  (The sum's chunks are cut at the gradients' boundaries, these at the outputs': at most
+// one more for each of the kPairTensors tensors.)
 constexpr int kJoinedChunks = 512;
+static_assert(kJoinedChunks + kPairTensors <= kWideThreads, "a thread per partial sum");
 template <typename T, typename L>
 __global__ __launch_bounds__(kWideThreads) void scale_joined_kernel(L list, const double *__restrict__ partial, int count,
                                                                     void *norm, int f64, double max_norm) {

@@ -3,7 +3,8 @@ and for the exact gradient of a batch's tables, which is never stored -- the fus
 
 Squares are added up in 64 bits and the norm is rounded once, to float32 (float64 if a gradient is float64); the
 scale is min(1, max_norm / (norm + 1e-6)).  Nothing synchronises unless a caller asks for an error: the norm is
-a tensor on the device.  Checks and outputs are those of the compiled module (table_batched_embeddings_cpp) over
+a tensor on the device.  Like torch.nn.utils.clip_grad_norm_, these functions take no part in autograd: norms carry
+no graph.  Checks and outputs are those of the compiled module (table_batched_embeddings_cpp) over
 the C-ABI library (include/tbe_hip.h).
 """
 import torch

@@ -25,7 +25,8 @@ def expert_plan(expert_ids, num_experts):
 
 def expert_dispatch(tokens, places, expert_offsets):
     """The rows of `tokens` ([tokens, D]) in expert order: row places[t, j] is tokens[t]; zeros behind the
-    last expert's rows.  Differentiable with respect to `tokens`, once (a token's gradient is the sum of its
+    last expert's rows.  `places` is a plan's: every row is named once (rows that a caller's own places leave out
+    are not written, and of two pairs that name one row either may win).  Differentiable with respect to `tokens`, once (a token's gradient is the sum of its
     kept rows', added up in 32 bits, or 64 for float64)."""
     return compiled().expert_dispatch(tokens, places, expert_offsets)
 
@@ -33,7 +34,7 @@ def expert_dispatch(tokens, places, expert_offsets):
 def expert_combine(rows, places, expert_offsets, weights=None):
     """[tokens, D]: the sum over a token's kept pairs of weights[t, j] * rows[places[t, j]] (weights None:
     ones), added up in 32 bits (64 for float64) and rounded once.  Differentiable with respect to `rows` and
-    `weights` (float32, or the rows' dtype), once."""
+    `weights` (float32, or the rows' dtype), once; the gradient takes `places` for a plan's, as expert_dispatch does."""
     return compiled().expert_combine(rows, places, expert_offsets, weights)
 
 

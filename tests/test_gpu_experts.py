@@ -421,3 +421,15 @@ def test_a_layer_on_top_of_embedding_bags(fp16):
     moved = bags.embedding_weights.detach().double().cpu() - start.detach()
     step_rounding = torch.finfo(dtype).eps / 2 * start.detach().abs().max() * np.sqrt(start.numel())
     assert float((moved + 0.1 * table.grad).norm()) <= tol * float(0.1 * table.grad.norm()) + float(step_rounding)
+
+
+def test_forward_mode_derivatives_are_refused():
+    ids = torch.tensor([[0, 1], [1, 0]], device=DEV)
+    routing = ops.ExpertRouting(ids, 2)
+    x, rows, gates = torch.ones(2, 8, device=DEV), torch.ones(4, 8, device=DEV), torch.ones(2, 2, device=DEV)
+    with torch.autograd.forward_ad.dual_level():
+        dual = lambda t: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: routing.dispatch(dual(x)), lambda: routing.combine(dual(rows), gates),
+                     lambda: routing.combine(rows, dual(gates))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
