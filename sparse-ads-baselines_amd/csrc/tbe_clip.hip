@@ -203,23 +203,25 @@ __global__ __launch_bounds__(kWideThreads) void scale_kernel(L list, const void 
     chunk_scaled<T, kWideThreads, 1, STREAM_IN, STREAM_OUT>(piece_of_chunk<T>(list, chunk), scale, threadIdx.x);
 }
 
-// The same behind a sum over at most kWideThreads workgroups: every workgroup adds up the partial sums itself, in the
-// same order, and the first one writes the norm, in place of a launch in between.  For lists whose workgroups all run at
-// once, two per compute unit.  (The sum's chunks are cut at the gradients' boundaries, these at the outputs': at most
-// one more for each of the kPairTensors tensors.)
-constexpr int kJoinedChunks = 512;
-static_assert(kJoinedChunks + kPairTensors <= kWideThreads, "a thread per partial sum");
-template <typename T, typename L>
-__global__ __launch_bounds__(kWideThreads) void scale_joined_kernel(L list, const double *__restrict__ partial, int count,
-                                                                    void *norm, int f64, double max_norm) {
+// The same where the caches hold the gradients: every workgroup adds up the partial sums itself, in the order of
+// norm_finish_kernel, and the first one writes the norm, in place of a launch in between.  Two workgroups per compute
+// unit, which all run at once, walk the chunks.  (fp32, scaled in place, this way and with that launch: 4 M elements
+// 14.8 and 16.3 us, 12 M 27.4 and 29.2, 60 M 141 and 144; within the limit 12 M 13.7 and 16.4, 60 M 48.6 and 58.7.)
+constexpr int kJoinedBlocks = 512;
+constexpr int64_t kJoinedSums = 4 * kWideThreads;  // (each of a long list of lists' launches would add up all of them)
+template <typename T, typename L, bool STREAM_OUT>
+__global__ __launch_bounds__(kWideThreads) void scale_joined_kernel(L list, const double *__restrict__ partial,
+                                                                    int64_t count, void *norm, int f64, double max_norm) {
   using A = typename AccOf<T>::type;
-  const double root = sqrt(block_sum<kWideThreads / kWave>(static_cast<int>(threadIdx.x) < count ? partial[threadIdx.x] : 0.0));
+  double sum = 0.0;
+  for (int64_t i = threadIdx.x; i < count; i += kWideThreads) sum += partial[i];
+  const double root = sqrt(block_sum<kWideThreads / kWave>(sum));
   const double n = f64 ? root : static_cast<double>(static_cast<float>(root));
   if (blockIdx.x == 0 && threadIdx.x == 0) store_norm(norm, f64, root);
   const A scale = static_cast<A>(clip_scale(n, max_norm));
   if (!L::kPairs && scale == A(1)) return;
   for (int chunk = blockIdx.x; chunk < list.chunks; chunk += gridDim.x)
-    chunk_scaled<T, kWideThreads, 1, false, false>(piece_of_chunk<T>(list, chunk), scale, threadIdx.x);
+    chunk_scaled<T, kWideThreads, 1, false, STREAM_OUT>(piece_of_chunk<T>(list, chunk), scale, threadIdx.x);
 }
 
 // Few chunks: norm and scaling in one workgroup, a wavefront per chunk.
@@ -610,6 +612,9 @@ uint64_t total_bytes(const ListCall &c) {
 // More than the 256 MB memory-side cache holds: the second pass finds little of what the first one read, so both are
 // streamed (1.2 GB squared and scaled: 558 us, 619 with plain accesses; 240 MB: 116 and 99 the other way round).
 bool streams(uint64_t bytes) { return bytes > (uint64_t{256} << 20); }
+// Outputs of their own push what the norm's pass has left out of the caches, unless they are streamed (240 MB: 63 us
+// a pass, 85 with plain stores); small ones are left to whoever reads them next.
+bool streams_out(bool same, uint64_t bytes) { return streams(bytes) || (!same && bytes > (uint64_t{32} << 20)); }
 
 // The partial sums of all lists; returns their number.
 int64_t launch_squares(const ListCall &c, double *partial, hipStream_t s) {
@@ -617,7 +622,8 @@ int64_t launch_squares(const ListCall &c, double *partial, hipStream_t s) {
   const bool stream = streams(total_bytes(c));
   for (const int32_t dtype : kDtypes) {
     for_lists<ReadList>(c, dtype, [&](const ReadList &list) {
-      const dim3 grid(static_cast<unsigned>(std::min(list.chunks, kMaxBlocks))), block(kBlockThreads);
+      const dim3 grid(static_cast<unsigned>(std::min(list.chunks, stream ? kMaxBlocks : kWideThreads))),
+          block(kBlockThreads);
       with_type(dtype, [&](auto t) {
         using T = decltype(t);
         if (stream) TBE_LAUNCH("gradient_squares", s, (square_sum_kernel<T, true>), grid, block, list, partial + used);
@@ -629,9 +635,7 @@ int64_t launch_squares(const ListCall &c, double *partial, hipStream_t s) {
   return used;
 }
 
-void launch_norm(const ListCall &c, void *workspace, void *norm, int32_t norm_dtype, hipStream_t s) {
-  double *partial = static_cast<double *>(workspace);
-  const int64_t used = launch_squares(c, partial, s);
+void launch_finish(const double *partial, int64_t used, void *norm, int32_t norm_dtype, hipStream_t s) {
   TBE_LAUNCH("gradient_norm", s, norm_finish_kernel, dim3(1), dim3(kWideThreads), partial, used, norm,
              norm_dtype == TBE_DTYPE_F64 ? 1 : 0);
 }
@@ -640,9 +644,7 @@ void launch_scale(const ListCall &c, double max_norm, const void *norm, int32_t 
   const int f64 = norm_dtype == TBE_DTYPE_F64 ? 1 : 0;
   const uint64_t bytes = total_bytes(c);
   const bool same = in_place(c);
-  // Outputs of their own push what the norm's pass has left out of the caches, unless they are streamed (240 MB: 63 us
-  // a pass, 85 with plain stores); small ones are left to whoever reads them next.
-  const bool stream_in = streams(bytes), stream_out = stream_in || (!same && bytes > (uint64_t{32} << 20));
+  const bool stream_in = streams(bytes), stream_out = streams_out(same, bytes);
   for (const int32_t dtype : kDtypes) {
     with_type(dtype, [&](auto t) {
       using T = decltype(t);
@@ -659,10 +661,10 @@ void launch_scale(const ListCall &c, double max_norm, const void *norm, int32_t 
   }
 }
 
-// What a call's lists come to, for the forms that take one list.
+// What a call's lists come to.
 struct Lists {
   int32_t dtype = -1;     // -1: no elements; -2: several types
-  int64_t tensors = 0, chunks = 0;
+  int64_t chunks = 0;
   bool same;              // nothing is written, or in place
 };
 Lists count_lists(const ListCall &c) {
@@ -671,46 +673,53 @@ Lists count_lists(const ListCall &c) {
   for (int32_t i = 0; i < c.count; ++i) {
     if (c.numels[i] == 0) continue;
     l.dtype = l.dtype == -1 || l.dtype == c.dtypes[i] ? c.dtypes[i] : -2;
-    ++l.tensors;
     l.chunks += chunks_of(c.numels[i], reinterpret_cast<uint64_t>(l.same ? c.gradients[i] : c.outputs[i]), c.dtypes[i]).count;
   }
   return l;
-}
-
-// f(list) for the one list of a call whose tensors fit it.
-template <typename F> void for_one_list(const ListCall &c, const Lists &l, F &&f) {
-  if (l.same) for_lists<ReadList>(c, l.dtype, f);
-  else for_lists<PairList>(c, l.dtype, f);
 }
 
 // Norm (c.outputs null) or norm and scaling of one list of at most kFewChunks chunks, in one launch; whether it was one.
 bool launch_few(const ListCall &c, const Lists &l, double max_norm, void *norm, int32_t norm_dtype, hipStream_t s) {
   if (l.dtype < 0 || l.chunks > kFewChunks) return false;
   with_type(l.dtype, [&](auto t) {
-    for_one_list(c, l, [&](const auto &list) {
+    const auto launch = [&](const auto &list) {
       TBE_LAUNCH("gradient_clip_few", s, (clip_few_kernel<decltype(t), std::decay_t<decltype(list)>>), dim3(1),
                  dim3(kWideThreads), list, c.outputs ? 1 : 0, norm, norm_dtype == TBE_DTYPE_F64 ? 1 : 0, max_norm);
-    });
+    };
+    if (l.same) for_lists<ReadList>(c, l.dtype, launch);
+    else for_lists<PairList>(c, l.dtype, launch);
   });
   return true;
 }
 
-// Norm and scaling of one list of at most kJoinedChunks chunks, in two launches; whether it was one.  (100 tensors of 100 k
-// fp32 elements in all, outputs of their own: a pass of 10.6 us, 15.1 with a launch for the norm in between.)
-bool launch_joined(const ListCall &c, const Lists &l, double max_norm, void *workspace, void *norm, int32_t norm_dtype,
-                   hipStream_t s) {
-  if (l.dtype < 0 || l.chunks > kJoinedChunks || l.tensors > (l.same ? kListTensors : kPairTensors)) return false;
+// Norm and scaling.  (The norm is written by every list's launch, the same value.)
+void launch_clip(const ListCall &c, const Lists &l, double max_norm, void *workspace, void *norm, int32_t norm_dtype,
+                 hipStream_t s) {
+  const uint64_t bytes = total_bytes(c);
   double *partial = static_cast<double *>(workspace);
   const int64_t used = launch_squares(c, partial, s);
-  with_type(l.dtype, [&](auto t) {
-    using T = decltype(t);
-    for_one_list(c, l, [&](const auto &list) {
-      TBE_LAUNCH("gradient_scale", s, (scale_joined_kernel<T, std::decay_t<decltype(list)>>),
-                 dim3(static_cast<unsigned>(list.chunks)), dim3(kWideThreads), list, partial, static_cast<int>(used), norm,
-                 norm_dtype == TBE_DTYPE_F64 ? 1 : 0, max_norm);
+  if (streams(bytes) || used == 0 || used > kJoinedSums) {
+    launch_finish(partial, used, norm, norm_dtype, s);
+    launch_scale(c, max_norm, norm, norm_dtype, s);
+    return;
+  }
+  const int f64 = norm_dtype == TBE_DTYPE_F64 ? 1 : 0;
+  const bool stream_out = streams_out(l.same, bytes);
+  for (const int32_t dtype : kDtypes) {
+    with_type(dtype, [&](auto t) {
+      using T = decltype(t);
+      const auto launch = [&](const auto &list) {
+        using L = std::decay_t<decltype(list)>;
+        const dim3 grid(static_cast<unsigned>(std::min(list.chunks, kJoinedBlocks))), block(kWideThreads);
+        if (stream_out)
+          TBE_LAUNCH("gradient_scale", s, (scale_joined_kernel<T, L, true>), grid, block, list, partial, used, norm, f64, max_norm);
+        else
+          TBE_LAUNCH("gradient_scale", s, (scale_joined_kernel<T, L, false>), grid, block, list, partial, used, norm, f64, max_norm);
+      };
+      if (l.same) for_lists<ReadList>(c, dtype, launch);
+      else for_lists<PairList>(c, dtype, launch);
     });
-  });
-  return true;
+  }
 }
 
 int check_norm(const char *name, const void *norm, int32_t norm_dtype) {
@@ -790,7 +799,10 @@ extern "C" int tbe_gradient_norm(const void *const *gradients, const int64_t *nu
   if (int rc = check_norm(name, norm, norm_dtype)) return rc;
   if (int rc = check_workspace(name, num_tensors, workspace, workspace_bytes)) return rc;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (!launch_few(c, count_lists(c), 0.0, norm, norm_dtype, s)) launch_norm(c, workspace, norm, norm_dtype, s);
+  if (!launch_few(c, count_lists(c), 0.0, norm, norm_dtype, s)) {
+    double *partial = static_cast<double *>(workspace);
+    launch_finish(partial, launch_squares(c, partial, s), norm, norm_dtype, s);
+  }
   return check_launch(name);
 }
 
@@ -821,11 +833,7 @@ extern "C" int tbe_clip_gradients(const void *const *gradients, void *const *out
   if (int rc = check_overlap(name, c)) return rc;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const Lists l = count_lists(c);
-  if (!launch_few(c, l, max_norm, norm, norm_dtype, s) &&
-      !launch_joined(c, l, max_norm, workspace, norm, norm_dtype, s)) {
-    launch_norm(c, workspace, norm, norm_dtype, s);
-    launch_scale(c, max_norm, norm, norm_dtype, s);
-  }
+  if (!launch_few(c, l, max_norm, norm, norm_dtype, s)) launch_clip(c, l, max_norm, workspace, norm, norm_dtype, s);
   return check_launch(name);
 }
 

@@ -478,3 +478,21 @@ def test_a_whole_training_step_with_experts_and_clipping():
         weights = 2 * 2.0 ** -24 * 0.01 * math.sqrt(got.numel()) if got is clipped[0] else 0.0
         step_rounding = 2.0 ** -24 * (float(want.norm()) + float(got.norm()))
         assert float((got - scale * want).norm()) <= 4 * 2.0 ** -24 * float(got.norm()) + 2 * step_rounding + weights
+
+
+@pytest.mark.parametrize("count,numel", [(321, 13), (2000, 700), (9000, 40)])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_lists_of_thousands_of_tensors(count, numel, in_place):
+    """More lists, and more partial sums, than the form without a launch for the norm takes."""
+    gen = torch.Generator(device=DEV).manual_seed(count)
+    flat = torch.randn(count * numel, device=DEV, generator=gen)
+    want_norm = flat.double().norm()
+    tensors = list(torch.split(flat.clone(), numel))
+    out = None if in_place else list(torch.split(torch.full_like(flat, float("nan")), numel))
+    norm = ops.clip_gradients(tensors, 2.0, out=out)
+    assert abs(float(norm) - float(want_norm)) <= 2.0 ** -23 * float(want_norm)  # one rounding, and sums in 64 bits
+    assert torch.equal(norm, ops.gradient_norm(list(torch.split(flat, numel))))
+    want = flat.double() * (2.0 / (norm.double() + 1e-6))
+    got = torch.cat(tensors if in_place else out).double()
+    # the scale's rounding to 32 bits and the product's
+    assert bool(((got - want).abs() <= 2.01 * 2.0 ** -24 * want.abs()).all())
