@@ -27,6 +27,7 @@ namespace {
 constexpr int kChunkVectors = 1024;  // 16 KB
 constexpr int kListTensors = 320;    // read, or scaled in place
 constexpr int kPairTensors = 192;    // with outputs of their own
+constexpr int kShortList = kWave;    // calls of up to so many tensors pass short lists, which a launch copies
 constexpr int kNoBoundary = 0x8000;
 template <int N, bool PAIRS> struct TensorList {
   static constexpr int kTensors = N;
@@ -38,6 +39,8 @@ template <int N, bool PAIRS> struct TensorList {
 };
 using ReadList = TensorList<kListTensors, false>;
 using PairList = TensorList<kPairTensors, true>;
+using ShortReadList = TensorList<kShortList, false>;
+using ShortPairList = TensorList<kShortList, true>;
 static_assert(sizeof(ReadList) < 3900 && sizeof(PairList) < 3900, "kernel arguments");
 
 // The tensor that a chunk belongs to: every lane looks at some of the ends.
@@ -171,8 +174,8 @@ __device__ __forceinline__ double clip_scale(double norm, double max_norm) {
 }
 
 // A grid that fills the chip once walks the chunks; a partial sum per workgroup.
-template <typename T, bool STREAM>
-__global__ __launch_bounds__(kBlockThreads) void square_sum_kernel(ReadList list, double *__restrict__ partial) {
+template <typename T, typename L, bool STREAM>
+__global__ __launch_bounds__(kBlockThreads) void square_sum_kernel(L list, double *__restrict__ partial) {
   double sum = 0.0;
   for (int chunk = blockIdx.x; chunk < list.chunks; chunk += gridDim.x)
     sum += chunk_squares<T, kBlockThreads, 4, STREAM>(piece_of_chunk<T>(list, chunk), threadIdx.x);
@@ -224,27 +227,32 @@ __global__ __launch_bounds__(kWideThreads) void scale_joined_kernel(L list, cons
     chunk_scaled<T, kWideThreads, 1, false, STREAM_OUT>(piece_of_chunk<T>(list, chunk), scale, threadIdx.x);
 }
 
-// Few chunks: norm and scaling in one workgroup, a wavefront per chunk.
-constexpr int kFewChunks = 32;
+// Few chunks: norm and scaling in one workgroup, two wavefronts per chunk (8 fp32 chunks: 4.2 us a pass, 5.0 with one
+// wavefront each, 4.6 with four).  In place, where most passes have nothing to write, it serves up to three chunks a
+// pair of wavefronts, with outputs of their own one: 11 chunks within the limit 5.4 us, 7.0 in two launches, 22 chunks
+// 6.9 and 7.0 to 9.0 (the host's part); written 8 chunks 6.7 and 7.4, 11 chunks 9.1 and 7.2.
+constexpr int kFewChunks = 24;
+constexpr int kFewWritten = 8;
 template <typename T, typename L>
 __global__ __launch_bounds__(kWideThreads) void clip_few_kernel(L list, int scaled, void *norm, int f64,
                                                                 double max_norm) {
   using A = typename AccOf<T>::type;
-  constexpr int kWaves = kWideThreads / kWave;
-  const int lane = threadIdx.x & (kWave - 1);
-  const int wave = threadIdx.x >> 6;
+  constexpr int kThreads = 2 * kWave;
+  constexpr int kGroups = kWideThreads / kThreads;
+  const int thread = threadIdx.x % kThreads;
+  const int group = threadIdx.x / kThreads;
   double sum = 0.0;
-  for (int chunk = wave; chunk < list.chunks; chunk += kWaves)
-    sum += chunk_squares<T, kWave, 8, false>(piece_of_chunk<T>(list, chunk), lane);
-  sum = block_sum<kWaves>(sum);
+  for (int chunk = group; chunk < list.chunks; chunk += kGroups)
+    sum += chunk_squares<T, kThreads, 8, false>(piece_of_chunk<T>(list, chunk), thread);
+  sum = block_sum<kWideThreads / kWave>(sum);
   const double root = sqrt(sum);
   if (threadIdx.x == 0) store_norm(norm, f64, root);
   if (!scaled) return;
   const double n = f64 ? root : static_cast<double>(static_cast<float>(root));
   const A scale = static_cast<A>(clip_scale(n, max_norm));
   if (!L::kPairs && scale == A(1)) return;
-  for (int chunk = wave; chunk < list.chunks; chunk += kWaves)
-    chunk_scaled<T, kWave, 8, false, false>(piece_of_chunk<T>(list, chunk), scale, lane);
+  for (int chunk = group; chunk < list.chunks; chunk += kGroups)
+    chunk_scaled<T, kThreads, 8, false, false>(piece_of_chunk<T>(list, chunk), scale, thread);
 }
 
 // --------------------------------------------------------------------- norm of the tables' gradient
@@ -534,6 +542,15 @@ template <typename L, typename F> void for_lists(const ListCall &c, int32_t dtyp
   if (tensors) emit();
 }
 
+// The lists of a call that reads, or scales in place, or (pairs) has outputs of its own.
+template <typename F> void each_list(const ListCall &c, int32_t dtype, bool pairs, F &&f) {
+  const bool small = c.count <= kShortList;
+  if (pairs && small) for_lists<ShortPairList>(c, dtype, f);
+  else if (pairs) for_lists<PairList>(c, dtype, f);
+  else if (small) for_lists<ShortReadList>(c, dtype, f);
+  else for_lists<ReadList>(c, dtype, f);
+}
+
 int check_list(const char *name, const ListCall &c, bool outputs) {
   TBE_REQUIRE(c.count >= 0, "%s: num_tensors must not be negative", name);
   TBE_REQUIRE(c.count == 0 || (c.gradients && c.numels && c.dtypes && (c.outputs || !outputs)),
@@ -621,13 +638,14 @@ int64_t launch_squares(const ListCall &c, double *partial, hipStream_t s) {
   int64_t used = 0;
   const bool stream = streams(total_bytes(c));
   for (const int32_t dtype : kDtypes) {
-    for_lists<ReadList>(c, dtype, [&](const ReadList &list) {
+    each_list(c, dtype, false, [&](const auto &list) {
+      using L = std::decay_t<decltype(list)>;
       const dim3 grid(static_cast<unsigned>(std::min(list.chunks, stream ? kMaxBlocks : kWideThreads))),
           block(kBlockThreads);
       with_type(dtype, [&](auto t) {
         using T = decltype(t);
-        if (stream) TBE_LAUNCH("gradient_squares", s, (square_sum_kernel<T, true>), grid, block, list, partial + used);
-        else TBE_LAUNCH("gradient_squares", s, (square_sum_kernel<T, false>), grid, block, list, partial + used);
+        if (stream) TBE_LAUNCH("gradient_squares", s, (square_sum_kernel<T, L, true>), grid, block, list, partial + used);
+        else TBE_LAUNCH("gradient_squares", s, (square_sum_kernel<T, L, false>), grid, block, list, partial + used);
       });
       used += grid.x;
     });
@@ -655,8 +673,7 @@ void launch_scale(const ListCall &c, double max_norm, const void *norm, int32_t 
         else if (stream_out) TBE_LAUNCH("gradient_scale", s, (scale_kernel<T, L, false, true>), grid, block, list, norm, f64, max_norm);
         else TBE_LAUNCH("gradient_scale", s, (scale_kernel<T, L, false, false>), grid, block, list, norm, f64, max_norm);
       };
-      if (same) for_lists<ReadList>(c, dtype, launch);
-      else for_lists<PairList>(c, dtype, launch);
+      each_list(c, dtype, !same, launch);
     });
   }
 }
@@ -678,16 +695,15 @@ Lists count_lists(const ListCall &c) {
   return l;
 }
 
-// Norm (c.outputs null) or norm and scaling of one list of at most kFewChunks chunks, in one launch; whether it was one.
+// Norm (c.outputs null) or norm and scaling of one list of few chunks, in one launch; whether it was one.
 bool launch_few(const ListCall &c, const Lists &l, double max_norm, void *norm, int32_t norm_dtype, hipStream_t s) {
-  if (l.dtype < 0 || l.chunks > kFewChunks) return false;
+  if (l.dtype < 0 || l.chunks > (l.same ? kFewChunks : kFewWritten)) return false;
   with_type(l.dtype, [&](auto t) {
     const auto launch = [&](const auto &list) {
       TBE_LAUNCH("gradient_clip_few", s, (clip_few_kernel<decltype(t), std::decay_t<decltype(list)>>), dim3(1),
                  dim3(kWideThreads), list, c.outputs ? 1 : 0, norm, norm_dtype == TBE_DTYPE_F64 ? 1 : 0, max_norm);
     };
-    if (l.same) for_lists<ReadList>(c, l.dtype, launch);
-    else for_lists<PairList>(c, l.dtype, launch);
+    each_list(c, l.dtype, !l.same, launch);
   });
   return true;
 }
@@ -716,8 +732,7 @@ void launch_clip(const ListCall &c, const Lists &l, double max_norm, void *works
         else
           TBE_LAUNCH("gradient_scale", s, (scale_joined_kernel<T, L, false>), grid, block, list, partial, used, norm, f64, max_norm);
       };
-      if (l.same) for_lists<ReadList>(c, dtype, launch);
-      else for_lists<PairList>(c, dtype, launch);
+      each_list(c, dtype, !l.same, launch);
     });
   }
 }
