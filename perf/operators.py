@@ -258,19 +258,12 @@ def _plain_table(state):
 
 
 # --------------------------------------------------------------------------------- the framework's
-_ops = None
-
-
 def _framework():
-    """The framework's module, imported once: a user's program does so when it starts."""
-    global _ops
-    if _ops is None:
-        package = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "sparse-ads-baselines_amd")
-        if package not in sys.path:
-            sys.path.insert(0, package)
-        import table_batched_embeddings_ops
-        _ops = table_batched_embeddings_ops
-    return _ops
+    package = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "sparse-ads-baselines_amd")
+    if package not in sys.path:
+        sys.path.insert(0, package)
+    import table_batched_embeddings_ops as ops
+    return ops
 
 
 def _own(state):
