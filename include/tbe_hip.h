@@ -238,6 +238,20 @@ TBE_API int tbe_backward_approx_adagrad(const void *grad_output, void *weights, 
                                         int32_t stochastic_rounding, uint64_t seed, uint64_t offset,
                                         void *workspace, uint64_t workspace_bytes, void *stream);
 
+/* tbe_backward_approx_adagrad of grad_output * (*gradient_factor), one fp32 value in device memory (NULL: one; F16
+ * only): the products are formed in 32 bits, so that they need not lie in the gradient's type.
+ * grad_per_sample_weights stays that of grad_output without the factor. */
+TBE_API int tbe_backward_approx_adagrad_scaled(const void *grad_output, const float *gradient_factor, void *weights,
+                                        int32_t dtype, int64_t total_rows, int64_t max_table_rows, int32_t D,
+                                        const int32_t *table_offsets, int32_t T,
+                                        const int32_t *indices, int64_t num_indices,
+                                        const int32_t *offsets, int32_t B,
+                                        const void *per_sample_weights, void *optimizer_state,
+                                        float learning_rate, float eps,
+                                        void *grad_per_sample_weights,
+                                        int32_t stochastic_rounding, uint64_t seed, uint64_t offset,
+                                        void *workspace, uint64_t workspace_bytes, void *stream);
+
 /* The backward in two calls, so that the integer half can overlap other work.
  * tbe_plan_batch runs the stages that depend on the indices only -- gradient rows, sort, run
  * boundaries (table_batched_embeddings_cuda.cu:1618-1655 and the head test :1523-1539) -- and
@@ -258,6 +272,14 @@ TBE_API int tbe_plan_batch(const int32_t *table_offsets, int32_t T,
 TBE_API int tbe_backward_planned(int32_t optimizer, const void *grad_output, void *weights, int32_t dtype,
                                  int64_t total_rows, int32_t D, int32_t T, int32_t B, int64_t num_indices,
                                  const void *per_sample_weights, void *optimizer_state,
+                                 float learning_rate, float eps, void *grad_per_sample_weights,
+                                 int32_t stochastic_rounding, uint64_t seed, uint64_t offset,
+                                 void *workspace, uint64_t workspace_bytes, void *stream);
+
+/* tbe_backward_planned of grad_output * (*gradient_factor), as in tbe_backward_approx_adagrad_scaled. */
+TBE_API int tbe_backward_planned_scaled(int32_t optimizer, const void *grad_output, const float *gradient_factor,
+                                 void *weights, int32_t dtype, int64_t total_rows, int32_t D, int32_t T, int32_t B,
+                                 int64_t num_indices, const void *per_sample_weights, void *optimizer_state,
                                  float learning_rate, float eps, void *grad_per_sample_weights,
                                  int32_t stochastic_rounding, uint64_t seed, uint64_t offset,
                                  void *workspace, uint64_t workspace_bytes, void *stream);
@@ -693,7 +715,8 @@ TBE_API int tbe_expert_combine_backward(const void *grad_output, int64_t grad_st
  * tbe_table_gradient_norm writes the norm of the exact gradient of a batch's tables -- one row per distinct
  * (table, index), the sum over its lookups of (per_sample_weights[p] *) grad_output[bag(p)] -- from the workspace
  * that tbe_plan_batch (same D, dtype, T, B and num_indices) has filled.  It leaves the plan as it is: a
- * tbe_backward_planned may follow, with the same or a scaled grad_output.
+ * tbe_backward_planned may follow, with the same or a scaled grad_output (F16: a strongly scaled one loses bits below
+ * 2^-14; tbe_backward_planned_scaled multiplies in 32 bits).
  */
 TBE_API uint64_t tbe_gradient_norm_workspace_bytes(int32_t num_tensors);
 TBE_API int tbe_gradient_norm(const void *const *gradients, const int64_t *numels, const int32_t *dtypes,

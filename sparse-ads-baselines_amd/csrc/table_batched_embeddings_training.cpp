@@ -12,6 +12,7 @@
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 
+#include <cmath>
 #include <limits>
 #include <tuple>
 #include <vector>
@@ -332,29 +333,44 @@ at::Tensor clip_gradients(const py::object &source, double max_norm, const py::o
 }
 
 // ------------------------------------------------------------------------ clipped table updates
-struct TableClip {
-  at::Tensor clipped, norm;
-};
 
-// The batch's plan into `ws`, the norm of the tables' exact gradient, and grad_output scaled by it.
-TableClip plan_and_clip(const at::Tensor &grad_output, const at::Tensor &weights, const at::Tensor &table_offsets,
-                        const at::Tensor &indices, const at::Tensor &offsets,
-                        const c10::optional<at::Tensor> &indice_weights, const Shape &s, int32_t dtype, double max_norm,
-                        const at::Tensor &ws) {
+// The batch's plan into `ws` and the norm of the tables' exact gradient.
+at::Tensor plan_and_norm(const at::Tensor &grad_output, const at::Tensor &weights, const at::Tensor &table_offsets,
+                         const at::Tensor &indices, const at::Tensor &offsets,
+                         const c10::optional<at::Tensor> &indice_weights, const Shape &s, int32_t dtype,
+                         const at::Tensor &ws) {
   const bool f64 = weights.scalar_type() == at::kDouble;
-  TableClip clip{empty_on(grad_output, grad_output.sizes(), grad_output.scalar_type()), empty_norm(weights, f64)};
+  at::Tensor norm = empty_norm(weights, f64);
   void *stream = stream_of(weights);
   const uint64_t bytes = static_cast<uint64_t>(ws.numel());
   check(tbe_plan_batch(table_offsets.data_ptr<int32_t>(), s.T, indices.data_ptr<int32_t>(), s.n,
                        offsets.data_ptr<int32_t>(), s.B, s.rows, max_table_rows(table_offsets, s.rows), s.D, dtype,
                        ws.data_ptr(), bytes, stream));
   check(tbe_table_gradient_norm(grad_output.data_ptr(), dtype, s.D, s.T, s.B, s.n, ptr(indice_weights), ws.data_ptr(),
-                                bytes, clip.norm.data_ptr(), norm_code(f64), stream));
-  const void *gradient = grad_output.data_ptr();
-  void *output = clip.clipped.data_ptr();
-  const int64_t numel = grad_output.numel();
-  check(tbe_scale_gradients(&gradient, &output, &numel, &dtype, 1, max_norm, clip.norm.data_ptr(), norm_code(f64), stream));
-  return clip;
+                                bytes, norm.data_ptr(), norm_code(f64), stream));
+  return norm;
+}
+
+// `gradient` scaled down to max_norm by a norm that is on the device.
+at::Tensor scaled(const at::Tensor &gradient, double max_norm, const at::Tensor &norm) {
+  at::Tensor out = empty_on(gradient, gradient.sizes(), gradient.scalar_type());
+  const void *from = gradient.data_ptr();
+  void *to = out.data_ptr();
+  const int64_t numel = gradient.numel();
+  const int32_t dtype = float_code(gradient, "grad_output");
+  check(tbe_scale_gradients(&from, &to, &numel, &dtype, 1, max_norm, norm.data_ptr(),
+                            norm_code(norm.scalar_type() == at::kDouble), stream_of(gradient)));
+  return out;
+}
+
+// Whether a scaled copy of an fp16 gradient is too coarse for the update, whatever the gradient's values.  Below 2^-14
+// fp16 has steps of 2^-24, so that scaling moves an element by up to 2^-25, always to the same side for equal elements:
+// n lookups of D columns move the tables' gradient by up to n * sqrt(D) * 2^-25 (all of them in one row; per-sample weights
+// of up to one), or make it vanish.  The copy serves where that is no more than max_norm * 2^-11, the half step that every
+// larger element may be off by; else the update takes the factor itself, in 32 bits, on the gradient as it came.
+bool copy_is_too_coarse(const at::Tensor &weights, const Shape &s, double max_norm) {
+  return weights.scalar_type() == at::kHalf &&
+         max_norm < static_cast<double>(s.n) * std::sqrt(static_cast<double>(s.D)) * 0x1p-14;
 }
 
 at::Tensor plan_scratch(const at::Tensor &weights, const Shape &s, int32_t dtype) {
@@ -373,12 +389,12 @@ std::tuple<at::Tensor, at::Tensor> clip_table_gradient(at::Tensor grad_output, a
   const int32_t dtype = dtype_code(weights);
   c10::DeviceGuard guard(weights.device());
   const at::Tensor ws = plan_scratch(weights, s, dtype);
-  const TableClip clip = plan_and_clip(grad_output, weights, table_offsets, indices, offsets, indice_weights, s, dtype,
-                                       max_norm, ws);
-  return {clip.clipped, clip.norm};
+  const at::Tensor norm = plan_and_norm(grad_output, weights, table_offsets, indices, offsets, indice_weights, s, dtype, ws);
+  return {scaled(grad_output, max_norm, norm), norm};
 }
 
-// backward_sgd / backward_exact_adagrad on the clipped gradient, one plan for the norm and the update.
+// backward_sgd / backward_exact_adagrad on the clipped gradient, one plan for the norm and the update, or
+// backward_approx_adagrad, which makes its own.
 at::Tensor backward_clipped(int64_t optimizer, at::Tensor grad_output, at::Tensor weights, at::Tensor table_offsets,
                             at::Tensor indices, at::Tensor offsets, c10::optional<at::Tensor> indice_weights,
                             c10::optional<at::Tensor> optimizer_state, double learning_rate, double eps,
@@ -387,8 +403,10 @@ at::Tensor backward_clipped(int64_t optimizer, at::Tensor grad_output, at::Tenso
   grad_output = check_grad(grad_output, weights, s);
   check_weights_of_lookups(indice_weights, weights, indices);
   TORCH_CHECK(max_norm >= 0.0, "max_norm must not be negative");
-  TORCH_CHECK(optimizer == TBE_OPT_SGD || optimizer == TBE_OPT_ROWWISE_ADAGRAD, "optimizer must be SGD or row-wise Adagrad");
-  const bool adagrad = optimizer == TBE_OPT_ROWWISE_ADAGRAD;
+  TORCH_CHECK(optimizer == TBE_OPT_SGD || optimizer == TBE_OPT_ROWWISE_ADAGRAD ||
+                  optimizer == TBE_OPT_APPROX_ROWWISE_ADAGRAD,
+              "optimizer must be SGD or a row-wise Adagrad");
+  const bool adagrad = optimizer != TBE_OPT_SGD;
   TORCH_CHECK(adagrad || !indice_weights.has_value(), "SGD takes no per-sample weights");
   TORCH_CHECK(!adagrad || optimizer_state.has_value(), "row-wise Adagrad needs its state");
   if (adagrad) check_state(*optimizer_state, weights);
@@ -398,17 +416,32 @@ at::Tensor backward_clipped(int64_t optimizer, at::Tensor grad_output, at::Tenso
   std::pair<uint64_t, uint64_t> stream_of_bits{0, 0};
   if (rounds) stream_of_bits = rounding_stream(weights);
   const at::Tensor ws = plan_scratch(weights, s, dtype);
-  const TableClip clip = plan_and_clip(grad_output, weights, table_offsets, indices, offsets, indice_weights, s, dtype,
-                                       max_norm, ws);
+  const at::Tensor norm = plan_and_norm(grad_output, weights, table_offsets, indices, offsets, indice_weights, s, dtype, ws);
+  const float *factor = nullptr;
+  at::Tensor one;
+  if (copy_is_too_coarse(weights, s, max_norm)) {
+    one = scaled(at::ones({1}, weights.options().dtype(at::kFloat)), max_norm, norm);
+    factor = one.data_ptr<float>();
+  } else {
+    grad_output = scaled(grad_output, max_norm, norm);
+  }
   // (the clipped gradient's dot products with the rows, which nobody asks for: the update writes them)
   c10::optional<at::Tensor> unused;
   if (indice_weights.has_value()) unused = at::empty_like(*indice_weights);
-  check(tbe_backward_planned(static_cast<int32_t>(optimizer), clip.clipped.data_ptr(), weights.data_ptr(), dtype, s.rows,
-                             s.D, s.T, s.B, s.n, ptr(indice_weights), adagrad ? optimizer_state->data_ptr() : nullptr,
-                             static_cast<float>(learning_rate), static_cast<float>(eps),
-                             const_cast<void *>(ptr(unused)), rounds ? 1 : 0, stream_of_bits.first,
-                             stream_of_bits.second, ws.data_ptr(), static_cast<uint64_t>(ws.numel()), stream_of(weights)));
-  return clip.norm;
+  if (optimizer == TBE_OPT_APPROX_ROWWISE_ADAGRAD)
+    check(tbe_backward_approx_adagrad_scaled(
+        grad_output.data_ptr(), factor, weights.data_ptr(), dtype, s.rows, max_table_rows(table_offsets, s.rows), s.D,
+        table_offsets.data_ptr<int32_t>(), s.T, indices.data_ptr<int32_t>(), s.n, offsets.data_ptr<int32_t>(), s.B,
+        ptr(indice_weights), optimizer_state->data_ptr(), static_cast<float>(learning_rate), static_cast<float>(eps),
+        const_cast<void *>(ptr(unused)), rounds ? 1 : 0, stream_of_bits.first, stream_of_bits.second, ws.data_ptr(),
+        static_cast<uint64_t>(ws.numel()), stream_of(weights)));
+  else
+    check(tbe_backward_planned_scaled(
+        static_cast<int32_t>(optimizer), grad_output.data_ptr(), factor, weights.data_ptr(), dtype, s.rows, s.D, s.T, s.B,
+        s.n, ptr(indice_weights), adagrad ? optimizer_state->data_ptr() : nullptr, static_cast<float>(learning_rate),
+        static_cast<float>(eps), const_cast<void *>(ptr(unused)), rounds ? 1 : 0, stream_of_bits.first,
+        stream_of_bits.second, ws.data_ptr(), static_cast<uint64_t>(ws.numel()), stream_of(weights)));
+  return norm;
 }
 
 }  // namespace

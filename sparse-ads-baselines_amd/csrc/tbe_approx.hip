@@ -109,10 +109,13 @@ __global__ __launch_bounds__(kBlockThreads) void approx_adagrad_kernel(
     const int32_t *__restrict__ grad_rows, const int32_t *__restrict__ segment_starts,
     int32_t *__restrict__ counters, int32_t *__restrict__ long_queue, int D, int group, float lr,
     float eps, MixedTables mt, StochasticRounding sr, const int32_t *__restrict__ only_rows,
-    const int32_t *__restrict__ unique_slots, T *__restrict__ cache_rows, int slot_D) {
+    const int32_t *__restrict__ unique_slots, T *__restrict__ cache_rows, int slot_D,
+    const float *__restrict__ gradient_factor) {
   using V = RowVec<T, VEC>;
   using A = typename V::A;
   using R = typename V::R;
+  const float factor = MIXED ? 1.0f : factor_of<T>(gradient_factor);
+  lr *= factor;
 
   const int lane = threadIdx.x & (kWave - 1);
   const int r = lane / group;
@@ -234,7 +237,7 @@ __global__ __launch_bounds__(kBlockThreads) void approx_adagrad_kernel(
             for (int i = 0; i < VEC; ++i) local += x.v[i] * x.v[i];
           }
         }
-        const A gss = group_sum_pow2<A>(local, group);
+        const A gss = group_sum_pow2<A>(local, group) * factor * factor;
         A mult = A(0);
         if (live) {
           const A wss = WEIGHTED ? gss * pw * pw : gss;
@@ -287,7 +290,7 @@ template <typename T, int VEC, bool WEIGHTED, bool MIXED>
 __global__ __launch_bounds__(kBlockThreads) void approx_lookup_norms_kernel(
     const T *__restrict__ grad_output, const T *__restrict__ psw, const int32_t *__restrict__ offsets,
     const int32_t *__restrict__ counters, typename AccOf<T>::type *__restrict__ lookup_wss, int B,
-    int T_tables, int D, int group, MixedTables mt) {
+    int T_tables, int D, int group, MixedTables mt, const float *__restrict__ gradient_factor) {
   using V = RowVec<T, VEC>;
   using A = typename V::A;
   int queued = counters[1];  // (one queue, or one per XCD)
@@ -320,7 +323,8 @@ __global__ __launch_bounds__(kBlockThreads) void approx_lookup_norms_kernel(
 #pragma unroll
     for (int i = 0; i < VEC; ++i) local += x.v[i] * x.v[i];
   }
-  const A gss = group_sum_pow2<A>(local, group);
+  const float factor = MIXED ? 1.0f : factor_of<T>(gradient_factor);
+  const A gss = group_sum_pow2<A>(local, group) * factor * factor;
   for (int p = begin + c; p < end; p += group) {
     A wss = gss;
     if constexpr (WEIGHTED) {
@@ -460,6 +464,7 @@ template <typename T> struct LongRowArgs {
   const int32_t *unique_slots;  // cache-fronted tables: slot of each unique row (-1: not resident), or null
   T *cache_rows;
   int slot_D;  // elements of a cache row
+  const float *gradient_factor;
 };
 
 // First element of gradient row `grad_row` for a row at `p` (mixed-D tables: mt.T > 0).
@@ -1034,6 +1039,7 @@ __global__ __launch_bounds__(kBlockThreads) void approx_adagrad_long_kernel(
   // control flow and addressing stay scalar)
   const int lane = threadIdx.x & (kWave - 1);
   const int wave_in_block = uniform(static_cast<int>(threadIdx.x >> 6));
+  a.lr *= factor_of<T>(a.gradient_factor);
   // queue_capacity == 0: one queue, its length in counters[1] (mixed-D tables: and, from
   // mixed_huge_offset on, the rows of more than kApproxHuge occurrences that a workgroup walks, their
   // number in counters[xcd_counter(0)]).  Otherwise, as the short-row kernel
@@ -1208,6 +1214,7 @@ struct ApproxArgs {
   const int32_t *unique_slots;
   void *cache_rows;
   int32_t slot_D;
+  const float *gradient_factor;  // uniform tables only
 };
 
 template <typename T, int VEC>
@@ -1250,7 +1257,7 @@ void launch_approx(const ApproxArgs &a, const tbe_workspace_layout_t &l, char *w
   LongRowArgs<T> la{static_cast<const T *>(a.grad_output), static_cast<T *>(a.weights), static_cast<A *>(a.state),
                     static_cast<const T *>(a.psw), static_cast<T *>(a.grad_psw), i32(l.positions_sorted),
                     i32(l.grad_rows), lookup_wss, a.lr, a.eps, long_tables, a.sr, grad_bytes, a.unique_slots,
-                    static_cast<T *>(a.cache_rows), a.slot_D};
+                    static_cast<T *>(a.cache_rows), a.slot_D, a.gradient_factor};
   const bool big = grad_bytes >= (1ull << 32);
   const bool stochastic = sizeof(T) == 2 && a.sr.enabled;
 #define TBE_APPROX_LONG_KERNEL(WEIGHTED, STOCHASTIC, BIG)                                              \
@@ -1260,7 +1267,7 @@ void launch_approx(const ApproxArgs &a, const tbe_workspace_layout_t &l, char *w
 #define TBE_APPROX_LONG(WEIGHTED, MIXED)                                                               \
   TBE_LAUNCH("update_approx_norms", stream, (approx_lookup_norms_kernel<T, VEC, WEIGHTED, MIXED>),     \
              grid_norms, block, static_cast<const T *>(a.grad_output), static_cast<const T *>(a.psw),  \
-             a.offsets, counters, lookup_wss, a.B, a.T, a.D, group, a.mt);                             \
+             a.offsets, counters, lookup_wss, a.B, a.T, a.D, group, a.mt, a.gradient_factor);          \
   if (stochastic) {                                                                                    \
     if (big) { TBE_APPROX_LONG_KERNEL(WEIGHTED, sizeof(T) == 2, true); }                               \
     else { TBE_APPROX_LONG_KERNEL(WEIGHTED, sizeof(T) == 2, false); }                                  \
@@ -1274,7 +1281,7 @@ void launch_approx(const ApproxArgs &a, const tbe_workspace_layout_t &l, char *w
              static_cast<A *>(a.state), static_cast<const T *>(a.psw), static_cast<T *>(a.grad_psw),   \
              i32(l.keys_sorted), i32(l.positions_sorted), i32(l.grad_rows), i32(l.segment_starts),     \
              counters, long_queue, a.D, group, a.lr, a.eps, a.mt, a.sr, a.wide_rows, a.unique_slots,   \
-             static_cast<T *>(a.cache_rows), a.slot_D);                                                \
+             static_cast<T *>(a.cache_rows), a.slot_D, a.gradient_factor);                             \
   TBE_APPROX_LONG(WEIGHTED, MIXED)
   if (mixed) {
     if (a.psw) { TBE_APPROX(true, true); }
@@ -1304,6 +1311,7 @@ void launch_approx(const ApproxArgs &a, const tbe_workspace_layout_t &l, char *w
     ua.stochastic_rounding = a.sr;
     ua.unique_slots = a.unique_slots;
     ua.cache_rows = a.cache_rows;
+    ua.gradient_factor = a.gradient_factor;
     if (approx_sums_long_rows(a.dtype, a.D, a.psw != nullptr)) {
       // fp32 / fp64 rows without per-sample weights: the update of a row is a weighted sum of its
       // gradient rows, so the longer rows are summed in chunks like the exact update's
@@ -1315,7 +1323,7 @@ void launch_approx(const ApproxArgs &a, const tbe_workspace_layout_t &l, char *w
       (void)segment_update_approx_short(ua, nullptr, stream);
       TBE_LAUNCH("update_approx_norms", stream, (approx_lookup_norms_kernel<T, VEC, false, false>), grid_norms,
                  block, static_cast<const T *>(a.grad_output), static_cast<const T *>(nullptr), a.offsets, counters,
-                 lookup_wss, a.B, a.T, a.D, group, a.mt);
+                 lookup_wss, a.B, a.T, a.D, group, a.mt, static_cast<const float *>(nullptr));
       (void)segment_update_approx_sum_long(ua, lookup_wss, stream);
     } else {
       (void)segment_update_approx_short(ua, long_queue, stream);
@@ -1340,11 +1348,11 @@ int approx_update(const void *grad_output, void *weights, void *state, const voi
                   const int64_t *mixed_table_offsets, const int32_t *table_dim_offsets,
                   const int32_t *dim_offsets, int32_t total_D, int32_t T, const int32_t *offsets, int32_t B,
                   StochasticRounding sr, const tbe_workspace_layout_t &l, void *workspace, hipStream_t stream,
-                  const int32_t *unique_slots, void *cache_rows, int32_t slot_D) {
+                  const int32_t *unique_slots, void *cache_rows, int32_t slot_D, const float *gradient_factor) {
   ApproxArgs a{grad_output, weights, state, psw, grad_psw, dtype, fp16_vector_width, D, n, lr, eps,
                MixedTables{mixed_table_offsets, table_dim_offsets, dim_offsets, total_D, T}, sr, offsets, B, T,
                D == 0 ? approx_mixed_wide_queue(l, workspace) : nullptr, unique_slots, cache_rows,
-               D == 0 ? slot_D : D};
+               D == 0 ? slot_D : D, gradient_factor};
   char *ws = static_cast<char *>(workspace);
   // the queues of long rows borrow the chunk records' region: eight of approx_long_queue_capacity()
   // rows and one of the rows of more than kApproxHuge occurrences, or one queue of at most n / 9 rows
@@ -1376,8 +1384,22 @@ extern "C" int tbe_backward_approx_adagrad(const void *grad_output, void *weight
                                            void *grad_per_sample_weights,
                                            int32_t stochastic_rounding, uint64_t seed, uint64_t offset,
                                            void *workspace, uint64_t workspace_bytes, void *stream) {
+  return tbe_backward_approx_adagrad_scaled(grad_output, nullptr, weights, dtype, total_rows, max_table_rows, D,
+                                            table_offsets, T, indices, num_indices, offsets, B, per_sample_weights,
+                                            optimizer_state, learning_rate, eps, grad_per_sample_weights,
+                                            stochastic_rounding, seed, offset, workspace, workspace_bytes, stream);
+}
+
+extern "C" int tbe_backward_approx_adagrad_scaled(
+    const void *grad_output, const float *gradient_factor, void *weights, int32_t dtype, int64_t total_rows,
+    int64_t max_table_rows, int32_t D, const int32_t *table_offsets, int32_t T, const int32_t *indices,
+    int64_t num_indices, const int32_t *offsets, int32_t B, const void *per_sample_weights, void *optimizer_state,
+    float learning_rate, float eps, void *grad_per_sample_weights, int32_t stochastic_rounding, uint64_t seed,
+    uint64_t offset, void *workspace, uint64_t workspace_bytes, void *stream) {
   using namespace tbe;
   const char *name = "tbe_backward_approx_adagrad";
+  TBE_REQUIRE(!gradient_factor || dtype == TBE_DTYPE_F16, "%s: a gradient factor goes with fp16 tables (got dtype %d)",
+              name, dtype);
   TBE_REQUIRE(T > 0, "%s: T must be positive (got %d)", name, T);
   TBE_REQUIRE(B > 0, "%s: B must be positive (got %d)", name, B);
   TBE_REQUIRE(D > 0 && D % 4 == 0, "%s: D must be a positive multiple of 4 (got %d)", name, D);
@@ -1404,7 +1426,7 @@ extern "C" int tbe_backward_approx_adagrad(const void *grad_output, void *weight
   return approx_update(grad_output, weights, optimizer_state, per_sample_weights, grad_per_sample_weights,
                        dtype, g.vec, D, num_indices, learning_rate, eps, nullptr, nullptr, nullptr, 0, T, offsets, B,
                        StochasticRounding{seed, offset, (stochastic_rounding && dtype == TBE_DTYPE_F16) ? 1 : 0},
-                       l, workspace, s);
+                       l, workspace, s, nullptr, nullptr, 0, gradient_factor);
 }
 
 extern "C" int tbe_backward_approx_cached(const void *grad_output, const tbe_cache_t *cache, int32_t dtype,

@@ -183,6 +183,7 @@ struct BackwardCall {
   StochasticRounding stochastic_rounding;
   // interleaved tables [E][T][D]: entries of `offsets` per b (T or T + 1); 0 = table-major
   int32_t interleaved_offsets_stride = 0;
+  const float *gradient_factor = nullptr;  // as in UpdateArgs
 };
 
 int run_backward(const char *name, const BackwardCall &c) {
@@ -249,6 +250,7 @@ int run_backward(const char *name, const BackwardCall &c) {
   a.learning_rate = c.lr;
   a.eps = c.eps;
   a.stochastic_rounding = c.stochastic_rounding;
+  a.gradient_factor = c.gradient_factor;
   return segment_update(a, c.stream);
 }
 
@@ -485,16 +487,31 @@ extern "C" int tbe_backward_planned(int32_t optimizer, const void *grad_output, 
                                     float learning_rate, float eps, void *grad_per_sample_weights,
                                     int32_t stochastic_rounding, uint64_t seed, uint64_t offset,
                                     void *workspace, uint64_t workspace_bytes, void *stream) {
+  return tbe_backward_planned_scaled(optimizer, grad_output, nullptr, weights, dtype, total_rows, D, T, B, num_indices,
+                                     per_sample_weights, optimizer_state, learning_rate, eps, grad_per_sample_weights,
+                                     stochastic_rounding, seed, offset, workspace, workspace_bytes, stream);
+}
+
+extern "C" int tbe_backward_planned_scaled(int32_t optimizer, const void *grad_output, const float *gradient_factor,
+                                           void *weights, int32_t dtype, int64_t total_rows, int32_t D, int32_t T,
+                                           int32_t B, int64_t num_indices,
+                                           const void *per_sample_weights, void *optimizer_state,
+                                           float learning_rate, float eps, void *grad_per_sample_weights,
+                                           int32_t stochastic_rounding, uint64_t seed, uint64_t offset,
+                                           void *workspace, uint64_t workspace_bytes, void *stream) {
   using namespace tbe;
   TBE_REQUIRE(optimizer == TBE_OPT_SGD || optimizer == TBE_OPT_ROWWISE_ADAGRAD,
               "tbe_backward_planned: bad optimizer %d", optimizer);
   TBE_REQUIRE(optimizer != TBE_OPT_SGD || !per_sample_weights,
               "tbe_backward_planned: SGD takes no per-sample weights");
+  TBE_REQUIRE(!gradient_factor || dtype == TBE_DTYPE_F16,
+              "tbe_backward_planned: a gradient factor goes with fp16 tables (got dtype %d)", dtype);
   BackwardCall c{grad_output, weights, dtype, total_rows, 0, D, nullptr, T, nullptr, num_indices,
                  nullptr, B, per_sample_weights, optimizer_state, learning_rate, eps,
                  grad_per_sample_weights, workspace, workspace_bytes,
                  static_cast<hipStream_t>(stream),
                  optimizer == TBE_OPT_SGD ? kOptSgd : kOptAdagrad, true, nullptr, nullptr,
                  StochasticRounding{seed, offset, (stochastic_rounding && dtype == TBE_DTYPE_F16) ? 1 : 0}};
+  c.gradient_factor = gradient_factor;
   return run_backward("tbe_backward_planned", c);
 }

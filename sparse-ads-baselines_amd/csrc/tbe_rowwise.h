@@ -28,6 +28,14 @@ template <> __device__ __forceinline__ double approx_multiplier<double>(double s
   return weighted ? pw * static_cast<double>(lr) * inv : static_cast<double>(lr) * inv;
 }
 
+// A gradient in 16 bits may come with a factor, one value in device memory (null: none), that its type does not hold:
+// the learning rate takes the factor, a sum of the gradient's squares takes it twice, all in 32 bits.  (A factor of one
+// changes no bit; for the other types this is the constant.)
+template <typename T> __device__ __forceinline__ float factor_of(const float *gradient_factor) {
+  if constexpr (sizeof(T) == 2) return gradient_factor ? *gradient_factor : 1.0f;
+  else return 1.0f;
+}
+
 // v of the lane a data-parallel-primitive pattern selects, 0 where the pattern has no source lane
 // or the row mask leaves the lane out.
 template <int CTRL, int ROW_MASK> __device__ __forceinline__ float dpp_or_zero(float v) {

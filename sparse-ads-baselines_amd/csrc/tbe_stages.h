@@ -138,6 +138,7 @@ struct UpdateArgs {
   float learning_rate;
   float eps;
   StochasticRounding stochastic_rounding;  // fp16 weights only
+  const float *gradient_factor = nullptr;  // fp16 only: what grad_output is multiplied by (factor_of), null for one
 };
 
 int segment_update(const UpdateArgs &args, hipStream_t stream);
@@ -198,13 +199,14 @@ inline void set_bag_division(MixedTables &mt) {
 // mixed-D tables: D = 0, and the strip kernel of tbe_backward_mixed has already applied the rows
 // of few occurrences and filled the two queues above.  unique_slots / cache_rows (tables behind the
 // row cache; slot_D: the width of a cache row, for mixed-D tables): every row is updated where it
-// lives, as in segment_update.
+// lives, as in segment_update.  gradient_factor: as in UpdateArgs, for uniform tables.
 int approx_update(const void *grad_output, void *weights, void *state, const void *psw, void *grad_psw,
                   int32_t dtype, int32_t fp16_vector_width, int32_t D, int64_t n, float lr, float eps,
                   const int64_t *mixed_table_offsets, const int32_t *table_dim_offsets,
                   const int32_t *dim_offsets, int32_t total_D, int32_t T, const int32_t *offsets, int32_t B,
                   StochasticRounding sr, const tbe_workspace_layout_t &l, void *workspace, hipStream_t stream,
-                  const int32_t *unique_slots = nullptr, void *cache_rows = nullptr, int32_t slot_D = 0);
+                  const int32_t *unique_slots = nullptr, void *cache_rows = nullptr, int32_t slot_D = 0,
+                  const float *gradient_factor = nullptr);
 
 // Where the approximate update of mixed-D tables keeps its two queues of unique-row indices inside
 // the backward workspace: rows of at most 64 vectors with more occurrences than the strip kernel

@@ -45,14 +45,15 @@ __device__ __forceinline__ T *resolve_row(T *weights, T *cache_rows,
 
 // Applies the optimizer to one row held by a lane group.  `w_old` and `G` are
 // this lane's vector of the row; `state_old` is *state_row, read by the caller ahead of the
-// gradient sum so that its latency is off the row's critical path (unused for SGD).
+// gradient sum so that its latency is off the row's critical path (unused for SGD).  `factor`:
+// the gradient's (factor_of), which `lr` already carries.
 template <typename T, int VEC, int CHUNKS, int OPT, bool STREAMING = false>
 __device__ __forceinline__ void apply_update(T *wrow, const RowVec<T, VEC> &w_old,
                                              const RowVec<T, VEC> &G,
                                              typename AccOf<T>::type *state_row,
                                              typename AccOf<T>::type state_old, float lr,
                                              float eps, int chunks, int group_base, int c,
-                                             const StochasticRounding &sr, int64_t element) {
+                                             const StochasticRounding &sr, int64_t element, float factor) {
   using A = typename AccOf<T>::type;
   RowVec<T, VEC> w_new;
   if constexpr (OPT == kOptSgd) {
@@ -62,7 +63,7 @@ __device__ __forceinline__ void apply_update(T *wrow, const RowVec<T, VEC> &w_ol
     A local = A(0);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) local += G.v[i] * G.v[i];
-    const A gss = group_sum<CHUNKS, A>(local, chunks, group_base);
+    const A gss = group_sum<CHUNKS, A>(local, chunks, group_base) * factor * factor;
     const A s_new = state_old + gss;
     if (c == 0) *state_row = s_new;
     const A mult = adagrad_multiplier<A>(s_new, lr, eps);
@@ -102,7 +103,7 @@ __global__ __launch_bounds__(kBlockThreads) void update_short_kernel(
     ChunkRecord *__restrict__ chunk_records, int64_t max_chunks, int64_t max_long, int64_t n,
     int64_t num_tiles, int64_t tiles_per_xcd, int D_rt, int chunks_rt, float lr, float eps,
     const int32_t *__restrict__ unique_slots, T *__restrict__ cache_rows, StochasticRounding sr,
-    int32_t *__restrict__ approx_long_queue) {
+    int32_t *__restrict__ approx_long_queue, const float *__restrict__ gradient_factor) {
   using V = RowVec<T, VEC>;
   using A = typename V::A;
   // (a compile-time row width turns every row address into a shift)
@@ -148,6 +149,8 @@ __global__ __launch_bounds__(kBlockThreads) void update_short_kernel(
   const int u_limit = id_last + 1;
   const int nseg = u_limit - u_first;  // <= kTilePositions
   if (nseg <= 0) return;
+  const float factor = factor_of<T>(gradient_factor);
+  lr *= factor;
 
   // Bookkeeping into LDS.  All loads of one level are issued before the first dependent load:
   // the segment bounds, then -- both only need the bounds -- the keys and the tile's sorted
@@ -285,7 +288,7 @@ __global__ __launch_bounds__(kBlockThreads) void update_short_kernel(
             A local = A(0);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) local += x.v[i] * x.v[i];
-            const A gss = group_sum<CHUNKS, A>(local, chunks, group_base);
+            const A gss = group_sum<CHUNKS, A>(local, chunks, group_base) * factor * factor;
             A pw = A(1);
             if constexpr (WEIGHTED) pw = to_acc(pw_raw[q]);
             state_old = state_old + (WEIGHTED ? gss * pw * pw : gss);
@@ -331,7 +334,7 @@ __global__ __launch_bounds__(kBlockThreads) void update_short_kernel(
     w_old.unpack(w_raw);
     apply_update<T, VEC, CHUNKS, OPT, true>(wrow, w_old, G, state ? state + key : nullptr, state_old, lr,
                                             eps, chunks, group_base, c, sr,
-                                            static_cast<int64_t>(key) * D + col);
+                                            static_cast<int64_t>(key) * D + col, factor);
   }
 }
 
@@ -359,7 +362,7 @@ __global__ __launch_bounds__(kBlockThreads) void update_chunks_kernel(
     const ChunkRecord *__restrict__ chunk_records, int64_t max_chunks,
     typename AccOf<T>::type *__restrict__ partial_sums, int D_rt, int chunks_rt, float lr, float eps,
     const int32_t *__restrict__ unique_slots, T *__restrict__ cache_rows, StochasticRounding sr,
-    const int32_t *__restrict__ segment_starts) {
+    const int32_t *__restrict__ segment_starts, const float *__restrict__ gradient_factor) {
   using V = RowVec<T, VEC>;
   using A = typename V::A;
   // (a compile-time row width turns every row address into a shift)
@@ -398,6 +401,8 @@ __global__ __launch_bounds__(kBlockThreads) void update_chunks_kernel(
   const int64_t stride = static_cast<int64_t>(gridDim.x / kNumXcd) * kWavesPerBlock;
   int64_t g = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + (threadIdx.x >> 6);
   const int64_t shared_stride = static_cast<int64_t>(gridDim.x) * kWavesPerBlock;
+  const float factor = factor_of<T>(gradient_factor);
+  lr *= factor;
 
   while (true) {
     const ChunkRecord *next;
@@ -549,7 +554,7 @@ __global__ __launch_bounds__(kBlockThreads) void update_chunks_kernel(
       } else {
         apply_update<T, VEC, CHUNKS, OPT>(wrow, w_old, G, state ? state + rec.key : nullptr, state_old,
                                           lr, eps, chunks, 0, c, sr,
-                                          static_cast<int64_t>(rec.key) * D + col);
+                                          static_cast<int64_t>(rec.key) * D + col, factor);
       }
     }
   }
@@ -597,7 +602,7 @@ __global__ __launch_bounds__(kBlockThreads) void update_long_finish_kernel(
     const int32_t *__restrict__ counters, const LongRecord *__restrict__ long_records,
     const typename AccOf<T>::type *__restrict__ partial_sums, int D_rt, int chunks_rt, float lr,
     float eps, const int32_t *__restrict__ unique_slots, T *__restrict__ cache_rows,
-    StochasticRounding sr, int64_t max_long) {
+    StochasticRounding sr, int64_t max_long, const float *__restrict__ gradient_factor) {
   using V = RowVec<T, VEC>;
   using A = typename V::A;
   // (a compile-time row width turns every row address into a shift)
@@ -613,6 +618,8 @@ __global__ __launch_bounds__(kBlockThreads) void update_long_finish_kernel(
   const int64_t col = static_cast<int64_t>(c) * VEC;
   const int64_t wave_id = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + (threadIdx.x >> 6);
   const int64_t stride = static_cast<int64_t>(gridDim.x) * kWavesPerBlock;
+  const float factor = factor_of<T>(gradient_factor);
+  lr *= factor;
 
   for (int64_t slot = wave_id; slot < lists.total; slot += stride) {
     const LongRecord rec = long_record_at(long_records, lists, slot);
@@ -668,7 +675,7 @@ __global__ __launch_bounds__(kBlockThreads) void update_long_finish_kernel(
     }
     if (r == 0) {
       apply_update<T, VEC, CHUNKS, OPT>(wrow, w_old, G, state ? state + rec.key : nullptr, state_old, lr,
-                                        eps, chunks, 0, c, sr, static_cast<int64_t>(rec.key) * D + col);
+                                        eps, chunks, 0, c, sr, static_cast<int64_t>(rec.key) * D + col, factor);
     }
   }
 }
@@ -686,7 +693,7 @@ __global__ __launch_bounds__(kBlockThreads) void update_wide_kernel(
     const int32_t *__restrict__ positions_sorted, const int32_t *__restrict__ grad_rows,
     const int32_t *__restrict__ segment_starts, const int32_t *__restrict__ counters, int D,
     int chunks, float lr, float eps, const int32_t *__restrict__ unique_slots,
-    T *__restrict__ cache_rows, StochasticRounding sr) {
+    T *__restrict__ cache_rows, StochasticRounding sr, const float *__restrict__ gradient_factor) {
   using V = RowVec<T, VEC>;
   using A = typename V::A;
 
@@ -694,6 +701,8 @@ __global__ __launch_bounds__(kBlockThreads) void update_wide_kernel(
   const int U = counters[0];
   const int64_t wave_id = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + (threadIdx.x >> 6);
   const int64_t stride = static_cast<int64_t>(gridDim.x) * kWavesPerBlock;
+  const float factor = factor_of<T>(gradient_factor);
+  lr *= factor;
 
   for (int64_t u = wave_id; u < U; u += stride) {
     const int seg_begin = segment_starts[u];
@@ -736,7 +745,7 @@ __global__ __launch_bounds__(kBlockThreads) void update_wide_kernel(
 #pragma unroll
         for (int k = 0; k < VEC; ++k) local += G.v[k] * G.v[k];
       }
-      const A gss = group_sum<kWave, A>(local, kWave, 0);
+      const A gss = group_sum<kWave, A>(local, kWave, 0) * factor * factor;
       const A s_new = state[row] + gss;
       if (lane == 0) state[row] = s_new;
       mult = adagrad_multiplier<A>(s_new, lr, eps);
@@ -791,7 +800,7 @@ void launch_narrow(const UpdateArgs &a, const RowGeometry &g, hipStream_t stream
              grid_short, block, go, w, st, psw, gpsw, a.keys_sorted, a.positions_sorted, a.grad_rows,       \
              a.segment_starts, a.segment_ids, a.counters, long_records, chunk_records, a.max_chunks,        \
              a.max_long, a.num_indices, num_tiles, tiles_per_xcd, a.D, g.chunks, a.learning_rate, a.eps,                \
-             a.unique_slots, cr, a.stochastic_rounding, static_cast<int32_t *>(nullptr))
+             a.unique_slots, cr, a.stochastic_rounding, static_cast<int32_t *>(nullptr), a.gradient_factor)
   if (small) { TBE_UPDATE_SHORT(true); }
   else { TBE_UPDATE_SHORT(false); }
 #undef TBE_UPDATE_SHORT
@@ -806,13 +815,13 @@ void launch_narrow(const UpdateArgs &a, const RowGeometry &g, hipStream_t stream
              grid_chunks, block,
              go, w, st, psw, gpsw, a.positions_sorted, a.grad_rows, a.counters, chunk_records,
              a.max_chunks, partial, a.D, g.chunks, a.learning_rate, a.eps, a.unique_slots, cr,
-             a.stochastic_rounding, static_cast<const int32_t *>(nullptr));
+             a.stochastic_rounding, static_cast<const int32_t *>(nullptr), a.gradient_factor);
 
   const int64_t want_long = ceil_div(a.max_long, kWavesPerBlock);
   const dim3 grid_finish(static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(want_long, 256 * 4))));
   TBE_LAUNCH("update_long_finish", stream, (update_long_finish_kernel<T, VEC, CHUNKS, OPT>),
              grid_finish, block, w, st, a.counters, long_records, partial, a.D, g.chunks,
-             a.learning_rate, a.eps, a.unique_slots, cr, a.stochastic_rounding, a.max_long);
+             a.learning_rate, a.eps, a.unique_slots, cr, a.stochastic_rounding, a.max_long, a.gradient_factor);
 }
 
 // The short-row kernel alone, in its per-lookup (approximate Adagrad) form; rows of more than
@@ -838,7 +847,8 @@ void launch_approx_short(const UpdateArgs &a, const RowGeometry &g, int32_t *que
              reinterpret_cast<ChunkRecord *>(a.chunk_segments), a.max_chunks, a.max_long, a.num_indices,        \
              num_tiles,                                                                                         \
              tiles_per_xcd, a.D, g.chunks, a.learning_rate, a.eps, a.unique_slots,                              \
-             static_cast<T *>(a.cache_rows), a.stochastic_rounding, static_cast<int32_t *>(nullptr))
+             static_cast<T *>(a.cache_rows), a.stochastic_rounding, static_cast<int32_t *>(nullptr),            \
+             static_cast<const float *>(nullptr))
       if (small) { TBE_APPROX_SUM_SHORT(true); }
       else { TBE_APPROX_SUM_SHORT(false); }
 #undef TBE_APPROX_SUM_SHORT
@@ -856,7 +866,7 @@ void launch_approx_short(const UpdateArgs &a, const RowGeometry &g, int32_t *que
              kNumXcd * approx_long_queue_capacity(a.num_indices), int64_t{0}, a.num_indices, num_tiles,         \
              tiles_per_xcd,                                                                                     \
              a.D, g.chunks, a.learning_rate, a.eps, a.unique_slots, static_cast<T *>(a.cache_rows),             \
-             a.stochastic_rounding, queue)
+             a.stochastic_rounding, queue, a.gradient_factor)
   if (small) { TBE_APPROX_SHORT(true); }
   else { TBE_APPROX_SHORT(false); }
 #undef TBE_APPROX_SHORT
@@ -886,7 +896,7 @@ void launch_geometry(const UpdateArgs &a, const RowGeometry &g, hipStream_t stre
                static_cast<const T *>(a.per_sample_weights),
                static_cast<T *>(a.grad_per_sample_weights), a.keys_sorted, a.positions_sorted,
                a.grad_rows, a.segment_starts, a.counters, a.D, g.chunks, a.learning_rate, a.eps,
-               a.unique_slots, static_cast<T *>(a.cache_rows), a.stochastic_rounding);
+               a.unique_slots, static_cast<T *>(a.cache_rows), a.stochastic_rounding, a.gradient_factor);
     return;
   }
   switch (g.tmpl) {
@@ -956,13 +966,13 @@ void launch_approx_sum_long(const UpdateArgs &a, const RowGeometry &g, const voi
                static_cast<const T *>(a.grad_output), w, st, static_cast<const T *>(lookup_wss),
                static_cast<T *>(nullptr), a.positions_sorted, a.grad_rows, a.counters, chunk_records, a.max_chunks,
                partial, a.D, g.chunks, a.learning_rate, a.eps, a.unique_slots, static_cast<T *>(a.cache_rows),
-               a.stochastic_rounding, a.segment_starts);
+               a.stochastic_rounding, a.segment_starts, static_cast<const float *>(nullptr));
     const int64_t want_long = ceil_div(a.max_long, kWavesPerBlock);
     const dim3 grid_finish(static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(want_long, 256 * 4))));
     // (the partial rows already carry the multipliers: the row takes their sum as it is)
     TBE_LAUNCH("update_long_finish", stream, (update_long_finish_kernel<T, VEC, CHUNKS, kOptSgd>), grid_finish,
                block, w, st, a.counters, long_records, partial, a.D, g.chunks, 1.0f, a.eps, a.unique_slots,
-               static_cast<T *>(a.cache_rows), a.stochastic_rounding, a.max_long);
+               static_cast<T *>(a.cache_rows), a.stochastic_rounding, a.max_long, static_cast<const float *>(nullptr));
     TBE_LAUNCH("update_approx_state", stream, (approx_long_state_kernel<A>), grid_finish, block, st,
                static_cast<const A *>(lookup_wss), a.positions_sorted, a.segment_starts, a.counters, long_records,
                a.max_long);

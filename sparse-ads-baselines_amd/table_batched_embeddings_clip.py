@@ -57,6 +57,9 @@ def clip_table_gradient(grad_output, weights, table_offsets, indices, offsets, m
     """For a batch of TableBatchedEmbeddingBags: (grad_output scaled, norm).  The norm is that of the tables'
     exact gradient -- for every distinct (table, index) the sum over its lookups of (indice_weights *)
     grad_output of the lookup's bag -- and the scaled grad_output is the one whose gradient has a norm of at most
-    max_norm."""
+    max_norm, up to the rounding of its elements to their type.  For fp16 that rounding counts: an element may be off
+    by half a step, 2**-11 of its value, and below 2**-14 by 2**-25 whatever its value, down to zero, so that a gradient
+    scaled far down, and summed over many lookups of a row, may exceed max_norm or vanish (a module's clip_gradient
+    does not go through such a copy)."""
     return compiled().clip_table_gradient(grad_output, weights, table_offsets, indices, offsets, max_norm,
                                           indice_weights)

@@ -94,7 +94,7 @@ class LookupFunction(torch.autograd.Function):
                                  Optimizer.EXACT_ROWWISE_ADAGRAD)
         plan, ctx.plan = ctx.plan, None
         if ctx.clip is not None:
-            ctx.clip.update(ctx, grad_output, L_max)
+            ctx.clip.update(ctx, grad_output)
             grad_per_sample_weight = None
         elif plan is not None:
             assert ctx.optimizer != Optimizer.SGD or per_sample_weights is None
@@ -128,7 +128,9 @@ class LookupFunction(torch.autograd.Function):
 class TableGradientClip:
     """Clips the exact gradient of a module's tables to a norm, inside backward, before the fused update.
     `norm` is the norm that the last backward's gradient had (a 0-dim tensor on the device), None before the
-    first."""
+    first.  The update is that of clip_table_gradient's scaled gradient, but for fp16 tables and limits below
+    lookups * sqrt(D) * 2**-14: there the rounding of a scaled fp16 gradient could move the norm by more than fp16's
+    half step, and the update multiplies grad_output, as it came, in 32 bits."""
 
     def __init__(self, max_norm):
         self.max_norm = float(max_norm)
@@ -136,17 +138,10 @@ class TableGradientClip:
         if not self.max_norm >= 0.0:
             raise RuntimeError("max_norm must not be negative")
 
-    def update(self, ctx, grad_output, L_max):
+    def update(self, ctx, grad_output):
         (weights, table_offsets, indices, offsets, per_sample_weights, optimizer_state) = ctx.saved_tensors
-        if ctx.optimizer == Optimizer.APPROX_ROWWISE_ADAGRAD:
-            # (the per-lookup update makes its own plan)
-            grad_output, self.norm = clip_table_gradient(grad_output, weights, table_offsets, indices, offsets,
-                                                         self.max_norm, per_sample_weights)
-            extension.backward_approx_adagrad(
-                grad_output, weights, table_offsets, indices, offsets, per_sample_weights, optimizer_state,
-                ctx.learning_rate, ctx.eps, L_max, ctx.stochastic_rounding, 1)
-            return
-        code = tbe_native.OPT_SGD if ctx.optimizer == Optimizer.SGD else tbe_native.OPT_ROWWISE_ADAGRAD
+        code = {Optimizer.SGD: tbe_native.OPT_SGD, Optimizer.EXACT_ROWWISE_ADAGRAD: tbe_native.OPT_ROWWISE_ADAGRAD,
+                Optimizer.APPROX_ROWWISE_ADAGRAD: tbe_native.OPT_APPROX_ROWWISE_ADAGRAD}[ctx.optimizer]
         self.norm = tbe_native.compiled().backward_clipped(
             code, grad_output, weights, table_offsets, indices, offsets, per_sample_weights, optimizer_state,
             ctx.learning_rate, ctx.eps or 0.0, ctx.stochastic_rounding, self.max_norm)

@@ -12,7 +12,7 @@ LIB_PATH = os.environ.get("TBE_HIP_LIBRARY") or os.path.join(_HERE, "libtbe_hip.
 
 DTYPE_F32, DTYPE_F16, DTYPE_F64 = 0, 1, 2
 DTYPE_BF16 = 3  # expert routing and gradient clipping only
-ABI_VERSION = 23
+ABI_VERSION = 24
 MAX_EXPERTS = 4095
 
 _c_i32p = ctypes.c_void_p
@@ -104,6 +104,8 @@ SIGNATURES = {
     "tbe_plan_batch": (ctypes.c_int, [_c_i32p, _i32, _c_i32p, _i64, _c_i32p, _i32, _i64, _i64, _i32, _i32, _vp, _u64, _vp]),
     "tbe_backward_planned": (ctypes.c_int, [_i32, _vp, _vp, _i32, _i64, _i32, _i32, _i32, _i64, _vp, _vp, _f32, _f32,
                                             _vp, _i32, _u64, _u64, _vp, _u64, _vp]),
+    "tbe_backward_planned_scaled": (ctypes.c_int, [_i32, _vp, _vp, _vp, _i32, _i64, _i32, _i32, _i32, _i64, _vp, _vp,
+                                                   _f32, _f32, _vp, _i32, _u64, _u64, _vp, _u64, _vp]),
     "tbe_linearize": (ctypes.c_int, [_c_i32p, _i32, _c_i32p, _i64, _c_i32p, _i32, _c_i32p, _c_i32p, _vp]),
     "tbe_forward_interleaved": (ctypes.c_int, [_vp, _i32, _i64, _i32, _i32, _c_i32p, _i64, _c_i32p, _i32, _i32, _vp,
                                                _vp]),
@@ -128,6 +130,9 @@ SIGNATURES = {
     "tbe_backward_approx_adagrad": (ctypes.c_int, [_vp, _vp, _i32, _i64, _i64, _i32, _c_i32p, _i32, _c_i32p, _i64,
                                                    _c_i32p, _i32, _vp, _vp, _f32, _f32, _vp, _i32, _u64, _u64, _vp,
                                                    _u64, _vp]),
+    "tbe_backward_approx_adagrad_scaled": (ctypes.c_int, [_vp, _vp, _vp, _i32, _i64, _i64, _i32, _c_i32p, _i32,
+                                                          _c_i32p, _i64, _c_i32p, _i32, _vp, _vp, _f32, _f32, _vp,
+                                                          _i32, _u64, _u64, _vp, _u64, _vp]),
     "tbe_cache_workspace_layout": (ctypes.c_int, [_i64, _i64, _i64, ctypes.POINTER(CacheWorkspaceLayout)]),
     "tbe_cache_init": (ctypes.c_int, [_cache_p, _vp]),
     "tbe_cache_prepare": (ctypes.c_int, [_cache_p, _i32, _i64, _i64, _i32, _c_i32p, _i32, _c_i32p, _i64, _c_i32p, _i32,
