@@ -556,6 +556,9 @@ template <typename T, typename W, int VEC> void launch_combine(const CombineCall
     if (stream) launch_combine_as<T, W, VEC, AHEAD, true>(c, output);               \
     else launch_combine_as<T, W, VEC, AHEAD, false>(c, output);                     \
   } while (0)
+    // as many rows ahead as a token has, in steps: a row ahead that is not there costs its request.  (2, 4 and 8 ahead,
+    // 32768 tokens, rows of 2048 bf16, one choice 43, 48 and 76 us, two 77, 77 and 96, three 93, 88 and 115, four 112, 111
+    // and 129, six 162, 167 and 163, eight 214, 211 and 211; 512 tokens, rows of 1024, eight choices 3.7, 3.2 and 3.2.)
     if (c.choices <= 2) TBE_COMBINE(2);
     else if (c.choices <= 4) TBE_COMBINE(4);
     else TBE_COMBINE(8);
@@ -563,6 +566,7 @@ template <typename T, typename W, int VEC> void launch_combine(const CombineCall
   }
 }
 
+constexpr int kWavefrontVectors = 352;  // widest row of a wavefront, see below
 template <typename T, typename W, int VEC, bool STREAM>
 void launch_combine_backward_as(const CombineCall &c, const void *grad, int64_t grad_stride, void *grad_rows,
                                 void *grad_weights) {
@@ -579,12 +583,14 @@ void launch_combine_backward_as(const CombineCall &c, const void *grad, int64_t 
              c.row_stride, c.places, c.kept, static_cast<const W *>(c.weights), static_cast<T *>(grad_rows),       \
              static_cast<W *>(grad_weights), static_cast<uint32_t>(pairs), slots, c.choices, vectors,              \
              static_cast<int>(c.D), magic, shift)
-  // (the narrowest group that holds a row; for rows of more than 256 vectors a workgroup: 16384 tokens, 4 rows of 512
-  // vectors each 232 us, a wavefront per row 250; for 256 vectors, 32768 tokens, 8 rows each, 463 and 447)
+  // The narrowest group that holds a row, a workgroup for rows of more than 352 vectors.  (A wavefront and a workgroup a
+  // row: 16384 tokens, 4 rows each, of 192 vectors 89 and 116 us, 257: 146 and 159, 288: 139 and 153, 352: 171 and 174,
+  // 384: 184 and 182, 448: 216 and 211, 512: 262 and 236, 1024: 508 and 493; 1024 tokens, 257: 8.4 and 9.4, 352: 10.4 and
+  // 11.4, 512: 14 and 16, 768: 19.5 and 19.0; 32 rows alone, which leave the chip empty, 257: 4.6 and 3.4.)
   if (vectors <= 8) { TBE_COMBINE_BACKWARD(8); }
   else if (vectors <= 16) { TBE_COMBINE_BACKWARD(16); }
   else if (vectors <= 32) { TBE_COMBINE_BACKWARD(32); }
-  else if (vectors <= 256) { TBE_COMBINE_BACKWARD(64); }
+  else if (vectors <= kWavefrontVectors) { TBE_COMBINE_BACKWARD(64); }
   else {
     slots = ceil_div(c.tokens, kNumXcd) * kNumXcd * c.choices;
     TBE_COMBINE_BACKWARD(256);
@@ -592,6 +598,8 @@ void launch_combine_backward_as(const CombineCall &c, const void *grad, int64_t 
 #undef TBE_COMBINE_BACKWARD
 }
 
+// (Streamed reads of the rows beyond what the memory-side cache holds, plain ones and these: 320 MB of rows of 2048 bf16
+// 155 and 147 us, 1 GB 472 and 469; 732 MB of rows of 64 fp32 431 and 419.)
 template <typename T, typename W, int VEC>
 void launch_combine_backward(const CombineCall &c, const void *grad, int64_t grad_stride, void *grad_rows,
                              void *grad_weights) {

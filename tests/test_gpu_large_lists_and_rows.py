@@ -109,6 +109,7 @@ def test_table_gradients_beyond_the_caches(dtype, B):
 
 # rows that fill whole 128-byte lines and rows that do not, for every lane group of combine's gradient, beyond 256 MB
 ROWS = [(BF16, 64, 2), (BF16, 128, 3), (F16, 256, 1), (BF16, 2048, 8), (F32, 1000, 4), (F64, 500, 2), (BF16, 2056, 4),
+        (BF16, 2816, 2), (F16, 2824, 3),
         (F32, 4096, 2), (BF16, 36, 5), (F16, 330, 2)]
 
 
@@ -193,7 +194,7 @@ def test_more_vectors_than_a_launch_numbers():
 
 
 # pairs beyond one round of the grid's 2^22 workgroups: a wavefront a pair (four a workgroup), and a workgroup a pair
-@pytest.mark.parametrize("pairs,D", [((1 << 24) + 77, 264), ((1 << 22) + 77, 2064)])
+@pytest.mark.parametrize("pairs,D", [((1 << 24) + 77, 264), ((1 << 22) + 77, 2840)])
 def test_combines_gradient_beyond_one_round_of_the_grid(pairs, D):
     needs(60)
     choices = 2
