@@ -653,8 +653,9 @@ TBE_API int tbe_backward_sgd_interleaved(const void *grad_output, void *weights,
  * The rows of tokens in the order of the experts they chose, and back: the routed part of a mixture-of-experts
  * layer.  No counterpart in the reference.  Token t of num_tokens chooses `choices` experts; pair
  * a = t * choices + j names its j-th.  A pair whose expert lies outside [0, num_experts) is dropped: it takes
- * part in nothing (its row, its weight and its gradient are not read), and its place is behind the last
- * expert's rows.  num_experts <= TBE_MAX_EXPERTS, num_tokens * choices < 2^31.
+ * part in nothing (what its row, its weight and its gradient hold, NaN among it, changes no result; its weight and
+ * row 0 may be read all the same and have to be readable), and its place is behind the last expert's rows.
+ * num_experts <= TBE_MAX_EXPERTS, num_tokens * choices < 2^31.
  *
  * tbe_expert_plan: a stable sort of the pairs by expert.
  *   expert_ids      int32 or int64 (id_bytes = 4 or 8) [num_pairs]
@@ -708,7 +709,8 @@ TBE_API int tbe_expert_combine_backward(const void *grad_output, int64_t grad_st
  *                        an infinite norm makes finite gradients zero.
  *   tbe_clip_gradients   the two in a row
  * outputs[i] may be gradients[i] (in place: nothing is written while the norm is within max_norm); any other
- * overlap of an output with a tensor of the list is refused.  max_norm >= 0 (infinity: nothing is scaled).
+ * overlap of an output with a tensor of the list is refused.  max_norm >= 0 (infinity: nothing is scaled, unless the
+ * norm is not a number).
  * The workspace serves one call at a time.  The calls only launch kernels on `stream`; they can be captured
  * (the addresses and counts are part of the captured launches).
  *

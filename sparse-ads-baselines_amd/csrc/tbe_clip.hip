@@ -1,6 +1,7 @@
 // The global norm of gradients and clipping to it, for gfx950:
 //   norm    N = sqrt(sum over all tensors and elements of g^2)
-//   scaled  g * min(1, max_norm / (N + 1e-6)), a NaN of the quotient kept
+//   scaled  g * min(1, max_norm / (N + 1e-6)); a norm that is no number makes every element one, and an infinite one
+//           under an infinite limit scales nothing
 // and, for a sorted batch of embedding lookups, the norm of the tables' exact gradient, which has one row
 // per distinct index and is never stored:
 //   N = sqrt(sum over rows r of || sum over lookups p of row r of (w_p *) g[bag(p)] ||^2)
@@ -23,7 +24,7 @@ namespace {
 // 16-byte vectors.  Chunks begin at the first 16-byte boundary of the tensor that is written (read, for a sum): the
 // elements before it, fewer than a vector, belong to the first chunk, those behind the last whole vector to the
 // last one.  The other tensor of a pair may lie at any element's address, which the memory system takes.
-// An entry is 12 bytes (20 with an output of its own), so that 300 tensors take one launch a pass.
+// An entry is 12 bytes, 20 with an output of its own: a launch takes 320 tensors, or 192.
 constexpr int kChunkVectors = 1024;  // 16 KB
 constexpr int kListTensors = 320;    // read, or scaled in place
 constexpr int kPairTensors = 192;    // with outputs of their own

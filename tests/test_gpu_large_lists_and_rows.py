@@ -227,3 +227,13 @@ def test_nothing_is_written_where_an_error_was_asked_for():
     with pytest.raises(RuntimeError, match="not finite"):
         ops.clip_grad_norm_(parameters, 0.01, error_if_nonfinite=True)
     assert all(torch.equal(q.grad.view(torch.int32), b) for q, b in zip(parameters, bits))
+
+
+def test_an_infinite_limit_scales_nothing_but_where_the_norm_is_no_number():
+    inf, nan = float("inf"), float("nan")
+    for values, want in [([1.0, -inf, 3.0], [1.0, -inf, 3.0]), ([1.0, 2.0], [1.0, 2.0]), ([1.0, nan, inf], [nan] * 3)]:
+        for out in (None, torch.zeros(len(values), device=DEV)):
+            g = torch.tensor(values, device=DEV)
+            ops.clip_gradients([g], inf, out=None if out is None else [out])
+            got = g if out is None else out
+            torch.testing.assert_close(got.cpu(), torch.tensor(want), rtol=0, atol=0, equal_nan=True)
