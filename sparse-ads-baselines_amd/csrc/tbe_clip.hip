@@ -193,10 +193,11 @@ __global__ __launch_bounds__(kWideThreads) void norm_finish_kernel(const double 
   if (threadIdx.x == 0) store_norm(norm, f64, sqrt(sum));
 }
 
-// A vector per thread and chunk (reading and writing want many short requests: 427 us with four vectors a thread where
-// this takes 381, a copy of 1.2 GB), a workgroup walking every kScaleBlocks-th chunk.  The grid is what a call within the
-// limit pays for, in place: 600 M bf16 elements take 194 us with up to 16384 workgroups, 246 with one per chunk, 177 for
-// the norm alone; scaled they take 572 either way, 592 with 2048 workgroups.
+// A vector per thread and chunk (reading and writing want many short requests: 300 tensors of 300 M fp32 elements in all,
+// measured and scaled in place, 569 us, with four vectors a thread of smaller workgroups 602), a workgroup walking every
+// kScaleBlocks-th chunk.  The grid is what a call within the limit pays for, in place: 600 M bf16 elements take 196 us with
+// up to 16384 workgroups, 246 with one per chunk, 183 with 2048, 177 for the norm alone; scaled into others they take 568,
+// 579 and 601.
 template <typename T, typename L, bool STREAM_IN, bool STREAM_OUT>
 __global__ __launch_bounds__(kWideThreads) void scale_kernel(L list, const void *norm, int f64, double max_norm) {
   using A = typename AccOf<T>::type;
@@ -210,7 +211,8 @@ __global__ __launch_bounds__(kWideThreads) void scale_kernel(L list, const void 
 // The same where the caches hold the gradients: every workgroup adds up the partial sums itself, in the order of
 // norm_finish_kernel, and the first one writes the norm, in place of a launch in between.  Two workgroups per compute
 // unit, which all run at once, walk the chunks.  (fp32, scaled in place, this way and with that launch: 4 M elements
-// 14.8 and 16.3 us, 12 M 27.4 and 29.2, 60 M 141 and 144; within the limit 12 M 13.7 and 16.4, 60 M 48.6 and 58.7.)
+// 11.7 and 13.1 us, 12 M 26.7 and 28.5, 60 M 107.9 and 105.5; within the limit 4 M 7.9 and 10.6, 12 M 13.7 and 16.4, 60 M
+// 39.9 and 53.2.)
 constexpr int kJoinedBlocks = 512;
 constexpr int64_t kJoinedSums = 4 * kWideThreads;  // (each of a long list of lists' launches would add up all of them)
 template <typename T, typename L, bool STREAM_OUT>
@@ -230,8 +232,8 @@ __global__ __launch_bounds__(kWideThreads) void scale_joined_kernel(L list, cons
 
 // Few chunks: norm and scaling in one workgroup, two wavefronts per chunk (8 fp32 chunks: 4.2 us a pass, 5.0 with one
 // wavefront each, 4.6 with four).  In place, where most passes have nothing to write, it serves up to three chunks a
-// pair of wavefronts, with outputs of their own one: 11 chunks within the limit 5.4 us, 7.0 in two launches, 22 chunks
-// 6.9 and 7.0 to 9.0 (the host's part); written 8 chunks 6.7 and 7.4, 11 chunks 9.1 and 7.2.
+// pair of wavefronts, with outputs of their own one: 11 chunks within the limit 5.5 us, 7.4 in two launches, 24 chunks
+// 7.4 and 7.5, 32 chunks 9.0 and 7.4; written 8 chunks 6.9 and 7.5, 11 chunks 8.8 and 7.6.
 constexpr int kFewChunks = 24;
 constexpr int kFewWritten = 8;
 template <typename T, typename L>
@@ -628,10 +630,11 @@ uint64_t total_bytes(const ListCall &c) {
   return bytes;
 }
 // More than the 256 MB memory-side cache holds: the second pass finds little of what the first one read, so both are
-// streamed (1.2 GB squared and scaled: 558 us, 619 with plain accesses; 240 MB: 116 and 99 the other way round).
+// streamed (1.2 GB squared and scaled: 568 us, 629 with plain accesses; 240 MB 117 and 107 the other way round).
 bool streams(uint64_t bytes) { return bytes > (uint64_t{256} << 20); }
-// Outputs of their own push what the norm's pass has left out of the caches, unless they are streamed (240 MB: 63 us
-// a pass, 85 with plain stores); small ones are left to whoever reads them next.
+// Outputs of their own push what the norm's pass has left out of the caches, unless they are streamed (240 MB squared and
+// scaled: 112 us, 141 with plain stores, 160 MB 77 and 81, 40 to 128 MB no difference to 63 and 64; two sets of 96 MB in
+// turn 49 and 57); small ones are left to whoever reads them next.
 bool streams_out(bool same, uint64_t bytes) { return streams(bytes) || (!same && bytes > (uint64_t{32} << 20)); }
 
 // The partial sums of all lists; returns their number.

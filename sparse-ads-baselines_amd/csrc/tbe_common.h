@@ -286,8 +286,15 @@ __device__ __forceinline__ void store_pack(T *p, const Pack<T, VEC> &v) {
     *p = v.v[0];
   } else {
     Words16 *w = reinterpret_cast<Words16 *>(p);
-    if constexpr (STREAM) __builtin_nontemporal_store(__builtin_bit_cast(Words16, v), w);
-    else *w = __builtin_bit_cast(Words16, v);
+    Words16 x = __builtin_bit_cast(Words16, v);
+    if constexpr (STREAM) {
+      // (a register that the compiler knows nothing about: a store that it builds anew from computed elements, for
+      // instance as four floats, loses the hint)
+      asm volatile("" : "+v"(x));
+      __builtin_nontemporal_store(x, w);
+    } else {
+      *w = x;
+    }
   }
 }
 
