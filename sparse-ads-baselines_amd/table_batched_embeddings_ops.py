@@ -130,7 +130,7 @@ class TableGradientClip:
     `norm` is the norm that the last backward's gradient had (a 0-dim tensor on the device), None before the
     first.  The update is that of clip_table_gradient's scaled gradient, but for fp16 tables and limits below
     lookups * sqrt(D) * 2**-14: there the rounding of a scaled fp16 gradient could move the norm by more than fp16's
-    half step, and the update multiplies grad_output, as it came, in 32 bits."""
+    half step (at per-sample weights of up to one), and the update multiplies grad_output, as it came, in 32 bits."""
 
     def __init__(self, max_norm):
         self.max_norm = float(max_norm)
