@@ -365,12 +365,14 @@ at::Tensor scaled(const at::Tensor &gradient, double max_norm, const at::Tensor 
 
 // Whether a scaled copy of an fp16 gradient is too coarse for the update, whatever the gradient's values.  Below 2^-14
 // fp16 has steps of 2^-24, so that scaling moves an element by up to 2^-25, always to the same side for equal elements:
-// n lookups of D columns move the tables' gradient by up to n * sqrt(D) * 2^-25 (all of them in one row; per-sample weights
-// of up to one), or make it vanish.  The copy serves where that is no more than max_norm * 2^-11, the half step that every
-// larger element may be off by; else the update takes the factor itself, in 32 bits, on the gradient as it came.
-bool copy_is_too_coarse(const at::Tensor &weights, const Shape &s, double max_norm) {
+// n lookups of D columns move the tables' gradient by up to n * sqrt(D) * 2^-25 (all of them in one row) times the largest
+// per-sample weight, or make it vanish.  The copy serves where that is no more than max_norm * 2^-11, the half step that
+// every larger element may be off by; else the update takes the factor itself, in 32 bits, on the gradient as it came.  The
+// host does not know the weights: up to kLargestWeight is allowed for.
+constexpr double kLargestWeight = 32.0;
+bool copy_is_too_coarse(const at::Tensor &weights, const Shape &s, bool weighted, double max_norm) {
   return weights.scalar_type() == at::kHalf &&
-         max_norm < static_cast<double>(s.n) * std::sqrt(static_cast<double>(s.D)) * 0x1p-14;
+         max_norm < static_cast<double>(s.n) * std::sqrt(static_cast<double>(s.D)) * 0x1p-14 * (weighted ? kLargestWeight : 1.0);
 }
 
 at::Tensor plan_scratch(const at::Tensor &weights, const Shape &s, int32_t dtype) {
@@ -419,7 +421,7 @@ at::Tensor backward_clipped(int64_t optimizer, at::Tensor grad_output, at::Tenso
   const at::Tensor norm = plan_and_norm(grad_output, weights, table_offsets, indices, offsets, indice_weights, s, dtype, ws);
   const float *factor = nullptr;
   at::Tensor one;
-  if (copy_is_too_coarse(weights, s, max_norm)) {
+  if (copy_is_too_coarse(weights, s, indice_weights.has_value(), max_norm)) {
     one = scaled(at::ones({1}, weights.options().dtype(at::kFloat)), max_norm, norm);
     factor = one.data_ptr<float>();
   } else {

@@ -129,8 +129,9 @@ class TableGradientClip:
     """Clips the exact gradient of a module's tables to a norm, inside backward, before the fused update.
     `norm` is the norm that the last backward's gradient had (a 0-dim tensor on the device), None before the
     first.  The update is that of clip_table_gradient's scaled gradient, but for fp16 tables and limits below
-    lookups * sqrt(D) * 2**-14: there the rounding of a scaled fp16 gradient could move the norm by more than fp16's
-    half step (at per-sample weights of up to one), and the update multiplies grad_output, as it came, in 32 bits."""
+    lookups * sqrt(D) * 2**-14, 32 times that with per-sample weights: there the rounding of a scaled fp16 gradient
+    could move the norm by more than fp16's half step (at weights of up to 32), and the update multiplies grad_output,
+    as it came, in 32 bits."""
 
     def __init__(self, max_norm):
         self.max_norm = float(max_norm)

@@ -64,6 +64,23 @@ def test_a_hot_row_under_a_strong_clip(max_norm, optimizer, weighted, stochastic
     assert bool(((moved[2] - want).abs() <= 1.01 * error * abs(want)).all()), (float(moved[2, 0]), want)
 
 
+def test_per_sample_weights_make_the_rounding_larger():
+    """Weights of 30 and a limit of 500: scaled elements of 2.3e-6, 38.7 steps of fp16, would move the norm by 0.8 %."""
+    B, L, D, lr, eps, max_norm = 3001, 301, 64, 1.0, 0.01, 500.0
+    n = B * L
+    idx = torch.zeros(n, dtype=torch.int32, device=DEV)
+    off = torch.arange(0, n + 1, L, dtype=torch.int32, device=DEV)
+    go = torch.full((B, 1, D), 2.0 ** -10, device=DEV, dtype=torch.float16)
+    m = module(1, 2, D, "EXACT_ROWWISE_ADAGRAD", lr, eps, torch.zeros(2, D))
+    clip = m.clip_gradient(max_norm)
+    m(idx, off, torch.full((n,), 30.0, device=DEV, dtype=torch.float16)).backward(go)
+    G = n * 30.0 * 2.0 ** -10  # (whole multiples of 2^-9 below 2^24 of them: exact sums)
+    norm = G * math.sqrt(D)
+    assert abs(float(clip.norm) - norm) <= 2 * U * norm
+    state = (max_norm / (norm + 1e-6) * norm) ** 2
+    assert abs(float(m.optimizer_state[0]) - state) <= 1.01 * (D + 11) * U * state
+
+
 @pytest.mark.parametrize("optimizer,weighted", [("SGD", False), ("EXACT_ROWWISE_ADAGRAD", False),
                                                 ("EXACT_ROWWISE_ADAGRAD", True), ("APPROX_ROWWISE_ADAGRAD", False),
                                                 ("APPROX_ROWWISE_ADAGRAD", True)])
